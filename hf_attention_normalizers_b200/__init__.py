@@ -34,6 +34,7 @@ from .paged import (
     paged_triton_attention,
 )
 from .varlen import varlen_hopper_attention
+from . import serving
 
 __all__ = [
     "AttentionReplacementPolicy",

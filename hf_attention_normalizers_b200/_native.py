@@ -78,6 +78,28 @@ class PagedDesc(ctypes.Structure):
     ]
 
 
+class ChunkDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("normalizer", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("total_q", ctypes.c_int32),
+        ("max_len_q", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("max_len_k", ctypes.c_int32),
+        ("num_cache_tokens", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/hfan.h declares, with its ctypes signature.
 _T = HfanTensor
 _P = ctypes.c_void_p
@@ -91,6 +113,12 @@ SIGNATURES = {
     "hfan_paged_decode_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PagedDesc)]),
     "hfan_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _T, _T, _T, _T, _P, _P, ctypes.c_int64, _P]),
     "hfan_paged_decode_static": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _T, _T, _T, _T, _P, _P]),
+    "hfan_paged_chunk_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ChunkDesc)]),
+    "hfan_paged_chunk_fwd": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _T, _T, _P, _P, ctypes.c_int64, _P]),
+    "hfan_paged_key_weights": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _P, _P, ctypes.c_int64, _P]),
+    "hfan_paged_append": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _T, _T, _P, ctypes.c_int64, _P]),
+    "hfan_paged_evict": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _P, ctypes.c_int64, ctypes.c_int32,
+                                        ctypes.c_int32, _P, _P, _P]),
     "hfan_rownorm_fwd": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
                                         _P, ctypes.c_int64, _P, ctypes.c_int64, _P]),
     "hfan_rownorm_bwd": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
@@ -100,7 +128,7 @@ SIGNATURES = {
     "hfan_abi_version": (ctypes.c_int, []),
 }
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 
 def library_path() -> str:

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "paged_serving.cuh"
 #include "params.cuh"
 
 namespace hfan {
@@ -275,6 +276,55 @@ int fill_paged(const hfan_paged_desc* desc, AttnParams& p) {
   return HFAN_OK;
 }
 
+// Fields of the serving requests that every entry point reads.
+int fill_chunk(const hfan_chunk_desc* desc, AttnParams& p) {
+  if (desc == nullptr) return fail(HFAN_ERR_INVALID, "null descriptor");
+  int rc = check_common(desc->dtype, desc->normalizer, desc->batch, desc->heads_q, desc->heads_kv, desc->head_dim);
+  if (rc != HFAN_OK) return rc;
+  if (desc->batch > 65535) return fail(HFAN_ERR_INVALID, "batch larger than 65535 is not supported (got %d)", desc->batch);
+  if (desc->heads_q > 65535) return fail(HFAN_ERR_INVALID, "more than 65535 heads are not supported (got %d)", desc->heads_q);
+  if (desc->page_size < 1) return fail(HFAN_ERR_INVALID, "block_size must be positive.");
+  if (desc->block_table == nullptr || desc->seq_lens == nullptr)
+    return fail(HFAN_ERR_INVALID, "block_table and sequence_lengths are required");
+  if (desc->total_q < 0 || desc->max_len_q < 0 || desc->max_len_k < 0 || desc->num_cache_tokens < 0)
+    return fail(HFAN_ERR_INVALID, "negative length");
+  if ((int64_t)desc->total_q * desc->heads_q > 2147483647ll)
+    return fail(HFAN_ERR_INVALID, "more than 2^31 - 1 (token, head) rows in one call");
+  if ((int64_t)desc->max_blocks * desc->page_size < desc->max_len_k)
+    return fail(HFAN_ERR_INVALID, "block_table does not contain enough blocks for sequence_lengths.");
+  p.batch = desc->batch;
+  p.hq = desc->heads_q;
+  p.hkv = desc->heads_kv;
+  p.d = desc->head_dim;
+  p.len_q = desc->max_len_q;
+  p.len_k = desc->max_len_k;
+  p.rows_total = desc->total_q;
+  p.cu_q = desc->cu_seqlens_q;
+  p.block_table = desc->block_table;
+  p.seq_lens = desc->seq_lens;
+  p.page_size = desc->page_size;
+  p.max_blocks = desc->max_blocks;
+  p.num_cache_tokens = desc->num_cache_tokens;
+  p.paged = 1;
+  p.scale = desc->scale;
+  p.causal = desc->causal ? 1 : 0;
+  p.norm = desc->normalizer;
+  return HFAN_OK;
+}
+
+int fill_chunk_rows(const hfan_chunk_desc* desc, AttnParams& p) {
+  int rc = fill_chunk(desc, p);
+  if (rc != HFAN_OK) return rc;
+  if (desc->cu_seqlens_q == nullptr) return fail(HFAN_ERR_INVALID, "cu_seqlens_q is required");
+  return HFAN_OK;
+}
+
+int check_weights(const hfan_chunk_desc* desc, const float* kw, int64_t ld) {
+  if (kw != nullptr && ld < desc->num_cache_tokens)
+    return fail(HFAN_ERR_INVALID, "key_weights must have a column for every cache slot.");
+  return HFAN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -437,6 +487,65 @@ int hfan_paged_decode_static(const hfan_paged_desc* desc, hfan_tensor q, hfan_te
   if (desc->max_len_k == 0) return HFAN_OK;
   e = decode_run(desc->dtype, p, desc->max_len_k, ws, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_decode_static");
+}
+
+int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc) {
+  AttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  if (fill_chunk_rows(desc, p) != HFAN_OK) return -1;
+  return 0;
+}
+
+int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, hfan_tensor value_cache,
+                         hfan_tensor o, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+  AttnParams p = base_params(q, key_cache, value_cache, o);
+  int rc = fill_chunk_rows(desc, p);
+  if (rc != HFAN_OK) return rc;
+  if (desc->total_q == 0 || desc->max_len_q == 0) return HFAN_OK;
+  if (stats == nullptr) return fail(HFAN_ERR_INVALID, "stats buffer is required");
+  p.stats = stats;
+  cudaError_t e = simt_attention_fwd(desc->dtype, p, desc->max_len_q, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_chunk_fwd");
+}
+
+int hfan_paged_key_weights(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, const float* stats,
+                           float* key_weights, int64_t ld_weights, void* stream) {
+  AttnParams p = base_params(q, key_cache, key_cache, q);
+  int rc = fill_chunk_rows(desc, p);
+  if (rc != HFAN_OK) return rc;
+  if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
+  if (desc->total_q == 0 || desc->max_len_q == 0 || desc->max_len_k == 0) return HFAN_OK;
+  if (stats == nullptr || key_weights == nullptr)
+    return fail(HFAN_ERR_INVALID, "stats and key_weights buffers are required");
+  p.stats = const_cast<float*>(stats);
+  cudaError_t e = serving_key_weights(desc->dtype, p, key_weights, ld_weights, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_key_weights");
+}
+
+int hfan_paged_append(const hfan_chunk_desc* desc, hfan_tensor k, hfan_tensor v, hfan_tensor key_cache,
+                      hfan_tensor value_cache, float* key_weights, int64_t ld_weights, void* stream) {
+  AttnParams p = base_params(k, key_cache, value_cache, v);
+  int rc = fill_chunk_rows(desc, p);
+  if (rc != HFAN_OK) return rc;
+  if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
+  if (desc->total_q == 0 || desc->max_len_k == 0) return HFAN_OK;
+  cudaError_t e = serving_append(desc->dtype, p, key_weights, ld_weights, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_append");
+}
+
+int hfan_paged_evict(const hfan_chunk_desc* desc, hfan_tensor key_cache, hfan_tensor value_cache, float* key_weights,
+                     int64_t ld_weights, int32_t budget, int32_t recent, int32_t* kept, int32_t* new_lens, void* stream) {
+  AttnParams p = base_params(key_cache, key_cache, value_cache, key_cache);
+  int rc = fill_chunk(desc, p);
+  if (rc != HFAN_OK) return rc;
+  if (key_weights == nullptr || kept == nullptr || new_lens == nullptr)
+    return fail(HFAN_ERR_INVALID, "key_weights, kept and new_lens buffers are required");
+  if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
+  if (budget < 1) return fail(HFAN_ERR_INVALID, "budget must be positive (got %d)", budget);
+  if (recent < 0) return fail(HFAN_ERR_INVALID, "recent must not be negative (got %d)", recent);
+  cudaError_t e = serving_evict(desc->dtype, p, key_weights, ld_weights, budget, recent, kept, new_lens,
+                                static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_evict");
 }
 
 int hfan_rownorm_fwd(int32_t normalizer, int32_t dtype, int64_t rows, int64_t n, const void* x,

@@ -1,0 +1,20 @@
+// Host entry points of the paged serving kernels.
+//
+// AttnParams fields as they are used here: cu_q [batch + 1] offsets of the
+// packed new tokens, rows_total their number, seq_lens / block_table /
+// page_size the cache's bookkeeping, len_k an upper bound of seq_lens.
+// Key weights are float32 [heads_kv][ld], one accumulator per cache slot.
+#pragma once
+
+#include "params.cuh"
+
+namespace hfan {
+
+// q = new K rows (q_st, q_sh), o = new V rows (o_st, o_sh) -> caches k, v.
+cudaError_t serving_append(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s);
+cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw, int budget, int recent, int* kept,
+                          int* new_lens, cudaStream_t s);
+// kw[kvh][slot] += sum of p over the chunk's rows of the KV group (p.stats: what the forward saved).
+cudaError_t serving_key_weights(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s);
+
+}  // namespace hfan

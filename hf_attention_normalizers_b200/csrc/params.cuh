@@ -122,7 +122,17 @@ __device__ __forceinline__ int seq_len_k(const AttnParams& p, int b) {
 
 __device__ __forceinline__ Geometry geometry(const AttnParams& p, int b) {
   Geometry g;
-  if (p.cu_q != nullptr) {
+  if (p.cu_q != nullptr && p.paged) {
+    // ragged chunk over a paged cache: nothing on the host has read the
+    // offsets, so they are clamped into the packed rows here
+    const int s = p.cu_q[b], e = p.cu_q[b + 1];
+    g.q_start = min(max(s, 0), p.rows_total);
+    const int end = min(max(e, g.q_start), p.rows_total);
+    g.q_len = end - g.q_start;
+    if ((g.q_start != s || end != e) && p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevBadLength);
+    g.k_start = 0;
+    g.k_len = seq_len_k(p, b);
+  } else if (p.cu_q != nullptr) {
     g.q_start = p.cu_q[b];
     g.q_len = p.cu_q[b + 1] - g.q_start;
     g.k_start = p.cu_k[b];

@@ -1,0 +1,189 @@
+"""Paged serving: one step of a batch whose sequences bring different numbers
+of new tokens, on a paged KV cache that is written and cut in place.
+
+A step calls, for every layer,
+
+* ``paged_append``           the new tokens' K/V rows go into their pages,
+* ``paged_chunk_attention``  the new tokens attend over the whole context (a
+  prompt piece, a single token, or a mix of them in one batch) and, on request,
+  add every key's attention weight to the cache's accumulators,
+* ``paged_evict``            when a sequence outgrew its budget: every KV head
+  keeps the keys with the most accumulated weight.
+
+Shapes (T new tokens of B sequences packed one after the other):
+
+* new rows ``[T, heads, dim]`` with ``cu_seqlens`` ``[B + 1]``; sequences may
+  bring no token;
+* caches ``[num_blocks * block_size, kv_heads, dim]``, any strides with a unit
+  innermost one (K and V may interleave in one allocation);
+* ``block_table`` ``[B, max_blocks]`` and ``sequence_lengths`` ``[B]``: the keys
+  of each sequence, its new tokens included, which are its last ones;
+* ``key_weights`` float32 ``[kv_heads, num_blocks * block_size]``: one
+  accumulator per KV head and cache slot.
+
+Inference only: nothing here has a gradient (``paged.paged_attention`` has).
+No call waits for the GPU; lengths, offsets and page ids are checked on the
+device, where a bad one is clamped or skipped and recorded in the status word
+that ``device_status`` reads.  ``max_seqlen_q`` / ``max_seqlen_k`` are upper
+bounds known to the host; without them the packed length and the block table's
+capacity are taken, which costs idle thread blocks.
+"""
+
+from __future__ import annotations
+
+from typing import Callable, Optional, Union
+
+import torch
+
+from . import _native as N
+from . import ops
+from .paged import _normalizer_name
+
+__all__ = ["paged_append", "paged_chunk_attention", "paged_evict", "device_status"]
+
+
+def _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights, name) -> None:
+    if key_cache.ndim != 3 or key_cache.shape != value_cache.shape:
+        raise ValueError("key_cache/value_cache must have matching [pages, heads, dim] shapes.")
+    if key_cache.dtype != value_cache.dtype:
+        raise ValueError("key_cache and value_cache must have one dtype.")
+    if key_cache.stride(2) != 1 or value_cache.stride(2) != 1:
+        raise ValueError("key_cache/value_cache must have a unit innermost stride.")
+    if not key_cache.is_cuda or not value_cache.is_cuda:
+        raise ValueError(f"{name} requires CUDA tensors.")
+    if block_table.ndim != 2:
+        raise ValueError("block_table must have shape [batch, max_blocks].")
+    if sequence_lengths.ndim != 1 or sequence_lengths.shape[0] != block_table.shape[0]:
+        raise ValueError("sequence_lengths must have shape [batch].")
+    if block_table.shape[0] < 1:
+        raise ValueError("The batch must hold at least one sequence.")
+    for t, what in ((block_table, "block_table"), (sequence_lengths, "sequence_lengths")):
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what} must use int32 or int64.")
+    if block_size <= 0:
+        raise ValueError("block_size must be positive.")
+    if key_weights is not None:
+        if key_weights.dtype != torch.float32 or key_weights.shape != (key_cache.shape[1], key_cache.shape[0]):
+            raise ValueError("key_weights must be float32 [kv_heads, num_blocks * block_size].")
+        if key_weights.stride(1) != 1 or key_weights.stride(0) < key_weights.shape[1]:
+            raise ValueError("key_weights must have contiguous rows.")
+
+
+def _check_rows(rows, key_cache, cu_seqlens, block_table, name) -> None:
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() != block_table.shape[0] + 1:
+        raise ValueError(f"{name} must have shape [batch + 1].")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must use int32 or int64.")
+    if rows.dtype != key_cache.dtype:
+        raise ValueError("New tokens and cache must have one dtype.")
+    if rows.shape[-1] != key_cache.shape[-1]:
+        raise ValueError("New tokens and cache head dimensions must match.")
+
+
+def _check_devices(first, *others) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("All tensors must be on one device.")
+    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+        raise ValueError("Paged serving is inference only: call it under torch.no_grad() or detach its inputs.")
+
+
+def _bound(given: Optional[int], most: int, name: str) -> int:
+    if given is None:
+        return most
+    if given < 0:
+        raise ValueError(f"{name} must not be negative.")
+    return min(int(given), most)
+
+
+def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                 block_table: torch.Tensor, cu_seqlens: torch.Tensor, sequence_lengths: torch.Tensor, block_size: int,
+                 key_weights: Optional[torch.Tensor] = None) -> None:
+    """Write the new tokens' ``[T, kv_heads, dim]`` K/V rows into the pages, in place.
+
+    Row ``i`` of the ``n`` new tokens of a sequence goes to its position
+    ``length - n + i``; the written slots of ``key_weights`` start at zero.
+    """
+    _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights, "paged_append")
+    if key.ndim != 3 or key.shape != value.shape:
+        raise ValueError("key/value must have matching [total_tokens, kv_heads, dim] shapes.")
+    if value.dtype != key.dtype:
+        raise ValueError("key and value must have one dtype.")
+    if key.shape[1] != key_cache.shape[1]:
+        raise ValueError("New keys and cache must have the same KV heads.")
+    _check_rows(key, key_cache, cu_seqlens, block_table, "cu_seqlens")
+    _check_devices(key_cache, value_cache, key, value, block_table, cu_seqlens, sequence_lengths, key_weights)
+    call = ops.paged_append if torch.compiler.is_compiling() else ops.launch_paged_append
+    call(key, value, key_cache, value_cache, block_table, cu_seqlens, sequence_lengths, int(block_size), key.shape[0],
+         key_weights)
+
+
+def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          block_table: torch.Tensor, cu_seqlens_q: torch.Tensor, sequence_lengths: torch.Tensor,
+                          block_size: int, normalizer: Union[str, Callable[..., torch.Tensor]] = "softmax1",
+                          scale: Optional[float] = None, is_causal: bool = True,
+                          key_weights: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None,
+                          max_seqlen_k: Optional[int] = None) -> torch.Tensor:
+    """Attention of a ragged chunk of new tokens ``[T, q_heads, dim]`` over the cached context.
+
+    The causal mask is aligned to each sequence's end (its new tokens are its
+    last keys); rows that see no key give zeros.  Cache slots past a sequence's
+    length are never used, whatever they hold.  With ``key_weights`` the
+    probabilities of every key, summed over the new tokens and the query heads
+    of its KV head, are added to its accumulator.
+    """
+    _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights,
+                 "paged_chunk_attention")
+    if query.ndim != 3:
+        raise ValueError("query must have shape [total_tokens, heads, dim].")
+    if query.shape[1] % key_cache.shape[1] != 0:
+        raise ValueError("query heads must be divisible by KV heads.")
+    _check_rows(query, key_cache, cu_seqlens_q, block_table, "cu_seqlens_q")
+    _check_devices(key_cache, value_cache, query, block_table, cu_seqlens_q, sequence_lengths, key_weights)
+    norm = N.NORMALIZER_IDS[_normalizer_name(normalizer)]
+    max_q = _bound(max_seqlen_q, query.shape[0], "max_seqlen_q")
+    max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
+    actual_scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
+    compiling = torch.compiler.is_compiling()
+    o, stats = (ops.paged_chunk_fwd if compiling else ops.launch_paged_chunk_fwd)(
+        query, key_cache, value_cache, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k, norm,
+        actual_scale, bool(is_causal))
+    if key_weights is not None:
+        (ops.paged_key_weights if compiling else ops.launch_paged_key_weights)(
+            query, key_cache, stats, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k, norm,
+            actual_scale, bool(is_causal), key_weights)
+    return o
+
+
+def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, key_weights: torch.Tensor,
+                block_table: torch.Tensor, sequence_lengths: torch.Tensor, block_size: int, budget: int,
+                recent: int = 0, max_seqlen_k: Optional[int] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence longer than ``budget`` to ``budget`` keys, per KV head and in place.
+
+    The ``recent`` last positions stay, the other places go to the largest
+    ``key_weights`` (ties to the lowest position).  What is kept moves, in
+    order, to the sequence's positions ``0 .. budget - 1``, so its pages past
+    ``ceil(budget / block_size)`` are free; slots past the budget keep what they
+    held.  The pages of a longer sequence must not be shared with another one.
+
+    Returns the new lengths ``int32 [B]`` and the former positions of what is
+    kept, ``int32 [B, kv_heads, budget]`` (-1 past a shorter sequence).
+    """
+    if key_weights is None:
+        raise ValueError("paged_evict requires key_weights.")
+    _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights, "paged_evict")
+    if budget < 1:
+        raise ValueError("budget must be positive.")
+    if recent < 0:
+        raise ValueError("recent must not be negative.")
+    _check_devices(key_cache, value_cache, block_table, sequence_lengths, key_weights)
+    max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
+    call = ops.paged_evict if torch.compiler.is_compiling() else ops.launch_paged_evict
+    return call(key_cache, value_cache, key_weights, block_table, sequence_lengths, int(block_size), max_k, int(budget),
+                int(recent))
+
+
+def device_status(clear: bool = True) -> int:
+    """Wait for the current stream and read the device status word: 0, or the first error the kernels
+    recorded (1: page id outside the cache, 2: a bounded wait ran out, 3: length or offset out of range)."""
+    return N.device_status(torch.cuda.current_stream().cuda_stream, clear)

@@ -46,7 +46,7 @@
 extern "C" {
 #endif
 
-#define HFAN_ABI_VERSION 2
+#define HFAN_ABI_VERSION 3
 
 typedef enum hfan_status {
   HFAN_OK = 0,
@@ -231,6 +231,71 @@ int hfan_paged_decode(const hfan_paged_desc* desc, hfan_tensor q, hfan_tensor ke
 int hfan_paged_decode_static(const hfan_paged_desc* desc, hfan_tensor q, hfan_tensor key_cache,
                              hfan_tensor value_cache, hfan_tensor o, float* stats, void* stream);
 
+/* ---- Paged serving: one step of a batch whose sequences bring different
+ * numbers of new tokens.  These entry points have no counterpart in the
+ * reference (its paged path takes one length for every sequence, and its cache
+ * neither writes in place nor evicts).
+ *
+ * Packed rows [total_q, heads, D]: sequence b owns rows cu_seqlens_q[b] ..
+ * cu_seqlens_q[b + 1] - 1, which are the last ones of its seq_lens[b] keys (so
+ * seq_lens counts the new tokens).  Caches are [num_cache_tokens, heads_kv, D]
+ * views (stride_batch ignored).  Key weights are float32 [heads_kv][ld]: one
+ * accumulator per KV head and cache slot, ld >= num_cache_tokens.
+ * The offsets and lengths stay on the device: out-of-range ones are clamped and
+ * recorded in the device status word (see hfan_device_status).  Sequences may
+ * bring no token; rows that see no key give a zero row. */
+typedef struct hfan_chunk_desc {
+  int32_t dtype;
+  int32_t normalizer;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t total_q;              /* packed new tokens                                     */
+  int32_t max_len_q;            /* upper bound of one sequence's new tokens              */
+  int32_t page_size;
+  int32_t max_blocks;           /* block_table row stride (columns)                      */
+  int32_t max_len_k;            /* upper bound of seq_lens                               */
+  int64_t num_cache_tokens;
+  const int32_t* block_table;   /* [batch, max_blocks] physical page ids                 */
+  const int32_t* cu_seqlens_q;  /* [batch + 1]                                           */
+  const int32_t* seq_lens;      /* [batch] keys of each sequence, the new ones included  */
+  float scale;
+  int32_t causal;               /* row i of n sees keys j <= len - n + i                 */
+} hfan_chunk_desc;
+
+/* Attention of the new tokens over the cached context.  q, o: packed views.
+ * stats: float32 [2, heads_q, total_q] as for hfan_attn_fwd.  workspace: device
+ * scratch of hfan_paged_chunk_workspace_bytes(desc) bytes, 256-byte aligned
+ * (NULL when that is 0). */
+int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc);
+int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, hfan_tensor value_cache,
+                         hfan_tensor o, float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* key_weights[kvh][slot] += the sum over the group's query heads and the new
+ * tokens of their probabilities on that key; q and stats as given to and
+ * written by hfan_paged_chunk_fwd.  A slot that is in one sequence's pages is
+ * added to once (the same bits on every run); slots of pages that several
+ * sequences share are added to once per sequence, in no fixed order. */
+int hfan_paged_key_weights(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, const float* stats,
+                           float* key_weights, int64_t ld_weights, void* stream);
+
+/* Writes the new tokens' K/V rows to their slots and zeroes the slots' key
+ * weights (key_weights may be NULL).  normalizer, heads_q and scale are ignored. */
+int hfan_paged_append(const hfan_chunk_desc* desc, hfan_tensor k, hfan_tensor v, hfan_tensor key_cache,
+                      hfan_tensor value_cache, float* key_weights, int64_t ld_weights, void* stream);
+
+/* Cuts every sequence longer than `budget` to `budget` keys, per KV head: the
+ * `recent` last positions stay (at most `budget` of them), the other places go
+ * to the largest key weights (ties to the lowest position; NaN counts as the
+ * largest).  The kept K, V and weights move, in order, to the sequence's
+ * positions 0 .. budget - 1; later positions keep what they held.  kept: int32
+ * [batch, heads_kv, budget] former positions (-1 past a shorter sequence);
+ * new_lens: int32 [batch].  Pages must belong to one sequence only.
+ * cu_seqlens_q, total_q, normalizer, heads_q and scale are ignored. */
+int hfan_paged_evict(const hfan_chunk_desc* desc, hfan_tensor key_cache, hfan_tensor value_cache, float* key_weights,
+                     int64_t ld_weights, int32_t budget, int32_t recent, int32_t* kept, int32_t* new_lens, void* stream);
+
 /* Row normalizers over the last axis of a [rows, n] matrix with row stride
  * ld (elements, unit column stride).  y/dx have the dtype of x. */
 int hfan_rownorm_fwd(int32_t normalizer, int32_t dtype, int64_t rows, int64_t n,
@@ -241,7 +306,8 @@ int hfan_rownorm_bwd(int32_t normalizer, int32_t dtype, int64_t rows, int64_t n,
 
 /* Synchronises `stream`, then reads the device status word of the current
  * device (0 = no error, 1 = out-of-range page id, 2 = bounded wait expired,
- * 3 = a sequence_lengths entry outside [0, max_len_k], clamped into that range)
+ * 3 = a sequence_lengths entry outside [0, max_len_k] or a cu_seqlens_q entry
+ * outside the packed rows, clamped into that range)
  * into *out; clear != 0 resets it. */
 int hfan_device_status(int* out, int clear, void* stream);
 

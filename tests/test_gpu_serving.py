@@ -1,0 +1,426 @@
+"""Paged serving operators (append, ragged chunk attention, key weights, eviction)
+against plain float64 implementations.
+
+Tolerances, from the formulas:
+  * a score s = scale q.k is a float32 sum of D exact products: the error of such a sum
+    is about sqrt(D) roundings of its largest partial sum, so |ds| <= DS =
+    4 sqrt(D) 2^-24 scale max sum|q_d k_d|;
+  * outputs: p is rounded to the 16-bit type before P V (relative U = 2^-9 for bfloat16,
+    2^-12 for float16, 0 for float32) and so is the result; a score error moves p by at most
+    2 DS dp/ds.  |do| <= 2 U sum p|v| + 2 DS sum g |v| + 1e-6 max|v|;
+  * key weights stay in float32: |dw| <= 2 DS sum g + 1e-6 w, summed over the rows,
+with g = dp/ds up to the threshold's own error: p (softmax1), 1[z > tau - 2 DS]
+(sparsemax), sqrt(p) + DS (entmax15).
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from hf_attention_normalizers_b200 import serving
+
+pytestmark = pytest.mark.gpu
+
+NORMS = ("softmax1", "sparsemax", "entmax15")
+UNIT = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -12, torch.bfloat16: 2.0 ** -9}
+
+
+class Batch:
+    """A paged cache with a ragged batch on it.  Slots that belong to no key hold NaN."""
+
+    def __init__(self, new, lens, *, hkv=2, group=4, dim=128, page=32, dtype=torch.bfloat16, seed=0, gain=1.0,
+                 interleave=False, extra_blocks=1, spare=2, stale=float("nan")):
+        g = torch.Generator().manual_seed(seed)
+        self.new, self.lens, self.hkv, self.group, self.dim, self.page, self.dtype = new, lens, hkv, group, dim, page, dtype
+        pages = [max(1, -(-c // page)) for c in lens]
+        order = torch.randperm(sum(pages) + spare, generator=g)
+        self.table = torch.full((len(lens), max(pages) + extra_blocks), -1, dtype=torch.int32)
+        self.rows = []
+        at = 0
+        for b, (n, c) in enumerate(zip(pages, lens)):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+            pos = torch.arange(c)
+            self.rows.append(self.table[b].long()[pos // page] * page + pos % page)
+        slots = (sum(pages) + spare) * page
+        kc = torch.full((slots, hkv, dim), stale)
+        vc = torch.full((slots, hkv, dim), stale)
+        for r in self.rows:
+            kc[r] = torch.randn(len(r), hkv, dim, generator=g)
+            vc[r] = torch.randn(len(r), hkv, dim, generator=g)
+        total = sum(new)
+        self.query = (torch.randn(total, hkv * group, dim, generator=g) * gain).to(dtype)
+        self.key_cache, self.value_cache = kc.to(dtype), vc.to(dtype)
+        self.weights = torch.rand(hkv, slots, generator=g)
+        self.cu = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32)
+        self.seq = torch.tensor(lens, dtype=torch.int32)
+        dev = "cuda"
+        self.d_query, self.d_table, self.d_cu, self.d_seq = (t.to(dev) for t in (self.query, self.table, self.cu, self.seq))
+        self.d_weights = self.weights.to(dev)
+        if interleave:  # K and V of a token side by side in one allocation
+            both = torch.stack((self.key_cache, self.value_cache), 1).to(dev)
+            self.d_key, self.d_value = both[:, 0], both[:, 1]
+        else:
+            self.d_key, self.d_value = self.key_cache.to(dev), self.value_cache.to(dev)
+
+    def chunk(self, norm, **kw):
+        kw.setdefault("max_seqlen_q", max(self.new))
+        kw.setdefault("max_seqlen_k", max(self.lens))
+        return serving.paged_chunk_attention(self.d_query, self.d_key, self.d_value, self.d_table, self.d_cu, self.d_seq,
+                                             self.page, normalizer=norm, **kw)
+
+    def expected(self, norm, causal=True, scale=None):
+        """Outputs, their tolerance, added key weights and their tolerance (float64)."""
+        scale = self.dim ** -0.5 if scale is None else scale
+        u = UNIT[self.dtype]
+        out = np.zeros(self.query.shape)
+        tol = np.zeros(self.query.shape)
+        add, add_tol = np.zeros(self.weights.shape), np.zeros(self.weights.shape)
+        q_all, kc, vc = self.query.double().numpy(), self.key_cache.double().numpy(), self.value_cache.double().numpy()
+        for b, (n, c) in enumerate(zip(self.new, self.lens)):
+            rows = self.rows[b].numpy()
+            for h in range(self.query.shape[1]):
+                kvh = h // self.group
+                k, v = kc[rows, kvh], vc[rows, kvh]
+                for i in range(n):
+                    t = int(self.cu[b]) + i
+                    see = min(c, c - n + i + 1) if causal else c
+                    if see <= 0:
+                        continue
+                    q = q_all[t, h]
+                    x = scale * (k[:see] @ q)
+                    p = oracle.normalize(norm, x[None])[0]
+                    ds = 4 * math.sqrt(self.dim) * 2.0 ** -24 * abs(scale) * (np.abs(k[:see]) @ np.abs(q)).max()
+                    if norm == "softmax1":
+                        g = p
+                    elif norm == "entmax15":
+                        g = np.sqrt(p) + ds
+                    else:
+                        tau = x[p > 0].min() - p[p > 0].min()
+                        g = (x > tau - 2 * ds).astype(np.float64)
+                    av = np.abs(v[:see])
+                    out[t, h] = p @ v[:see]
+                    tol[t, h] = 2 * u * (p @ av) + 2 * ds * (g @ av) + 1e-6 * av.max()
+                    add[kvh, rows[:see]] += p
+                    add_tol[kvh, rows[:see]] += 2 * ds * g + 1e-6 * p
+        return out, tol, add, add_tol
+
+
+def _check(actual, expected, tol, what):
+    a = actual.detach().double().cpu().numpy()
+    assert np.isfinite(a).all(), f"{what}: non-finite values"
+    over = np.abs(a - expected) - tol
+    assert over.max() <= 0, f"{what}: {over.max():.3e} over the tolerance, error {np.abs(a - expected).max():.3e}"
+
+
+def _chunk_case(batch, norm, causal=True, scale=None, **kw):
+    before = batch.weights.double().numpy()
+    out = batch.chunk(norm, is_causal=causal, scale=scale, key_weights=batch.d_weights, **kw)
+    want, tol, add, add_tol = batch.expected(norm, causal, scale)
+    _check(out, want, tol, f"{norm}/out")
+    # the accumulators themselves are float32
+    _check(batch.d_weights, before + add, add_tol + 1e-6 * (before + add), f"{norm}/weights")
+    assert serving.device_status() == 0
+
+
+SHAPES = [
+    # new, lens, layout
+    ([1], [1], {}),
+    ([1, 1, 1], [1, 33, 200], {}),
+    ([5], [5], dict(group=1)),
+    ([7, 0, 130], [40, 9, 131], {}),
+    ([3, 65, 1, 0], [3, 300, 257, 0], dict(group=5, hkv=1)),
+    ([64, 33], [64, 100], dict(group=7, hkv=2, dim=64)),
+    ([129], [700], dict(group=2, hkv=1, page=16)),
+    ([20, 1], [150, 1000], dict(group=8, hkv=2, dim=64, page=64)),
+    ([40], [383], dict(page=128)),
+    ([17, 9], [50, 270], dict(page=256, hkv=1)),
+    ([9, 4], [61, 44], dict(page=24, hkv=1)),
+    ([6, 2], [30, 77], dict(page=8, hkv=1)),
+    ([12], [45], dict(page=5, hkv=1)),
+    ([10, 3], [33, 90], dict(dim=40, hkv=1)),
+    ([3], [70], dict(group=48, hkv=1)),
+    ([2], [50], dict(group=160, hkv=1, dim=64)),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_chunk_attention_and_key_weights(case, norm, dtype):
+    new, lens, kw = SHAPES[case]
+    _chunk_case(Batch(new, lens, dtype=dtype, seed=case, gain=2.0, **kw), norm)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_chunk_without_causal_mask(norm):
+    _chunk_case(Batch([33, 4], [150, 40], seed=3), norm, causal=False)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.6])
+def test_chunk_scales(norm, scale):
+    """Equal scores (every key in the sparse support), negative and large scales."""
+    _chunk_case(Batch([20, 1], [500, 300], seed=4), norm, scale=scale)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_rows_without_a_visible_key_are_zero(norm):
+    """More new tokens than keys: the first rows see nothing."""
+    b = Batch([9, 140], [4, 130], seed=5)
+    _chunk_case(b, norm)
+    out = b.chunk(norm)
+    assert (out[:5] == 0).all() and (out[9:19] == 0).all() and out[5:9].abs().amax() > 0
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_interleaved_cache_strided_query_and_no_hints(norm):
+    b = Batch([30, 1, 70], [90, 257, 400], seed=6, interleave=True)
+    wide = torch.zeros(b.query.shape[0], b.query.shape[1], 3 * b.dim, dtype=b.dtype, device="cuda")
+    wide[..., b.dim:2 * b.dim] = b.d_query
+    b.d_query = wide[..., b.dim:2 * b.dim]
+    b.d_table, b.d_cu, b.d_seq = b.d_table.long(), b.d_cu.long(), b.d_seq.long()
+    _chunk_case(b, norm, max_seqlen_q=None, max_seqlen_k=None)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_unaligned_query_view(norm, dtype):
+    """A query view whose rows start off a 16-byte boundary."""
+    b = Batch([30, 5], [90, 41], seed=7, dtype=dtype)
+    wide = torch.zeros(b.query.shape[0], b.query.shape[1], b.dim + 3, dtype=b.dtype, device="cuda")
+    wide[..., 1:b.dim + 1] = b.d_query
+    b.d_query = wide[..., 1:b.dim + 1]
+    _chunk_case(b, norm)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_long_context_few_rows(norm):
+    """The key axis is split between thread blocks when there are few rows."""
+    _chunk_case(Batch([3, 1], [9001, 4100], seed=8, hkv=1, gain=2.0), norm)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_decode_batch(norm):
+    _chunk_case(Batch([1] * 5, [700, 1, 32, 1025, 64], seed=9, gain=2.0), norm)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_infinities_and_nan_outside_the_length(norm):
+    for stale in (float("inf"), -float("inf"), float("nan")):
+        _chunk_case(Batch([40, 2], [100, 70], seed=10, stale=stale), norm)
+
+
+def test_peaked_and_flat_rows_share_a_tile():
+    """Rows of one tile whose scores differ a lot in size: one key with everything beside even rows."""
+    for norm in NORMS:
+        b = Batch([32], [600], seed=11, hkv=1)
+        b.query[::2] *= 12.0
+        b.query[1::2] *= 0.01
+        b.d_query = b.query.cuda()
+        _chunk_case(b, norm)
+
+
+def test_same_bits_on_every_run():
+    for norm in NORMS:
+        outs = []
+        for _ in range(2):
+            b = Batch([100, 1, 30], [900, 3000, 300], seed=12)
+            outs.append((b.chunk(norm, key_weights=b.d_weights), b.d_weights))
+        assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_shared_pages_add_for_every_sequence(norm):
+    """Two sequences whose prefix is the same page: both add to its accumulators."""
+    b = Batch([4, 6], [64, 70], seed=13, hkv=1)
+    b.table[1, 0] = b.table[0, 0]
+    b.rows[1] = b.table[1].long()[torch.arange(70) // 32] * 32 + torch.arange(70) % 32
+    b.d_table = b.table.cuda()
+    _chunk_case(b, norm)
+
+
+def test_on_another_stream():
+    b = Batch([50, 3], [200, 90], seed=14)
+    ref = b.chunk("softmax1")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = b.chunk("softmax1")
+    side.synchronize()
+    assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 1, 200]])
+def test_in_a_cuda_graph(norm, new):
+    b = Batch(new, [500, 40, 1200], seed=15)
+    eager = b.chunk(norm, key_weights=b.d_weights)
+    w = b.weights.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b.chunk(norm, key_weights=w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager) and torch.equal(w, b.d_weights)
+
+
+def test_traced_by_compile():
+    b = Batch([5, 1], [80, 40], seed=16)
+
+    def step(q, kc, vc, w):
+        return serving.paged_chunk_attention(q, kc, vc, b.d_table, b.d_cu, b.d_seq, b.page, "entmax15", key_weights=w,
+                                             max_seqlen_q=5, max_seqlen_k=80) * 2
+
+    w = b.weights.cuda()
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(b.d_query, b.d_key, b.d_value, w)
+    want = step(b.d_query, b.d_key, b.d_value, b.d_weights)
+    assert torch.equal(got, want) and torch.equal(w, b.d_weights)
+
+
+def test_bad_page_and_length_are_recorded():
+    """A page id outside the cache reads as zeros, a length past the hint is clamped; both set the status word."""
+    for norm in NORMS:
+        b = Batch([20, 3], [100, 50], seed=17)
+        serving.device_status()
+        b.d_table[0, 1] = 10 ** 6
+        out = b.chunk(norm)
+        assert torch.isfinite(out).all() and serving.device_status() == 1 and serving.device_status() == 0
+        b.d_table.copy_(b.table)
+        b.chunk(norm, max_seqlen_k=90)
+        assert serving.device_status() == 3
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,offset", [(128, 0), (64, 0), (40, 0), (20, 0), (128, 1)])
+def test_append(dtype, dim, offset):
+    b = Batch([3, 0, 40, 1], [3, 9, 77, 33], dim=dim, dtype=dtype, seed=20, stale=7.0, interleave=dim == 64)
+    g = torch.Generator().manual_seed(1)
+    total = sum(b.new)
+    both = torch.randn(total, 2, b.hkv, dim + 2 * offset, generator=g).to(dtype)[..., offset:offset + dim]
+    kc, vc, kw = b.key_cache.clone(), b.value_cache.clone(), b.weights.clone()
+    for s, (n, c) in enumerate(zip(b.new, b.lens)):
+        rows, t = b.rows[s][c - n:], int(b.cu[s])
+        kc[rows], vc[rows], kw[:, rows] = both[t:t + n, 0], both[t:t + n, 1], 0.0
+    dev = torch.randn(total, 2, b.hkv, dim + 2 * offset).to(dtype).cuda()[..., offset:offset + dim]
+    dev.copy_(both)
+    serving.paged_append(dev[:, 0], dev[:, 1], b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page,
+                         key_weights=b.d_weights)
+    assert torch.equal(b.d_key.cpu(), kc) and torch.equal(b.d_value.cpu(), vc) and torch.equal(b.d_weights.cpu(), kw)
+    serving.paged_append(dev[:, 0], dev[:, 1], b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page)
+    assert torch.equal(b.d_weights.cpu(), kw) and serving.device_status() == 0
+
+
+def test_append_nothing_and_too_much():
+    b = Batch([0, 0], [5, 0], seed=21, stale=1.0)
+    kc = b.d_key.clone()
+    e = torch.zeros(0, b.hkv, b.dim, dtype=b.dtype, device="cuda")
+    serving.paged_append(e, e, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page)
+    assert torch.equal(b.d_key, kc) and serving.device_status() == 0
+    assert b.chunk("softmax1").shape == (0, 8, 128)
+    b = Batch([6], [4], seed=22)  # two more tokens than keys: they have no position
+    x = torch.randn(6, b.hkv, b.dim).to(b.dtype).cuda()
+    serving.paged_append(x, x, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page)
+    assert torch.equal(b.d_key[b.rows[0].cuda()], x[2:]) and serving.device_status() == 3
+
+
+# ---------------------------------------------------------------------------
+# evict
+# ---------------------------------------------------------------------------
+def _evict_expected(b, budget, recent):
+    kc, vc, kw = b.key_cache.clone(), b.value_cache.clone(), b.weights.clone()
+    kept = np.full((len(b.lens), b.hkv, budget), -1, dtype=np.int32)
+    for s, c in enumerate(b.lens):
+        for h in range(b.hkv):
+            if c <= budget:
+                kept[s, h, :c] = np.arange(c)
+                continue
+            late = min(recent, budget)
+            w = b.weights[h, b.rows[s]].double().numpy()[:c - late]
+            w = np.where(np.isnan(w), np.inf, w) + 0.0
+            nan = np.isnan(b.weights[h, b.rows[s]].numpy()[:c - late])
+            order = np.lexsort((np.arange(c - late), -w, ~nan))  # NaN first, then large weights, then low positions
+            keep = np.sort(np.concatenate([order[:budget - late], np.arange(c - late, c)]))
+            kept[s, h] = keep
+            dst, src = b.rows[s][:budget], b.rows[s][torch.from_numpy(keep)]
+            kc[dst, h], vc[dst, h], kw[h, dst] = b.key_cache[src, h], b.value_cache[src, h], b.weights[h, src]
+    return kept, kc, vc, kw
+
+
+def _evict_case(b, budget, recent, **kw_args):
+    kept, kc, vc, kw = _evict_expected(b, budget, recent)
+    lens, got = serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, budget, recent=recent,
+                                    **kw_args)
+    assert lens.tolist() == [min(c, budget) for c in b.lens]
+    np.testing.assert_array_equal(got.cpu().numpy(), kept)
+    for actual, want in ((b.d_key, kc), (b.d_value, vc), (b.d_weights, kw)):
+        np.testing.assert_array_equal(actual.float().cpu().numpy(), want.float().numpy())
+    assert serving.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("budget,recent", [(1, 0), (1, 1), (64, 0), (64, 17), (64, 64), (64, 100), (299, 5), (300, 0),
+                                           (1000, 10)])
+def test_evict(budget, recent, dtype):
+    _evict_case(Batch([1, 1, 1, 0, 1], [300, 64, 65, 0, 7], dtype=dtype, seed=30), budget, recent, max_seqlen_k=300)
+
+
+@pytest.mark.parametrize("kw", [dict(dim=64, page=16), dict(dim=40), dict(dim=20, page=5), dict(interleave=True), dict(hkv=1)])
+def test_evict_layouts(kw):
+    _evict_case(Batch([1, 1], [1500, 700], seed=31, **kw), 333, 20)
+
+
+def test_evict_ties_zeros_infinities_and_nan():
+    b = Batch([1, 1, 1], [2100, 2100, 500], seed=32)
+    w = torch.randint(0, 3, b.weights.shape, generator=torch.Generator().manual_seed(2)).float()  # many ties
+    w[:, b.rows[1]] = 0.0                                     # all equal
+    w[0, b.rows[1][5::7]] = -0.0                              # equal to +0
+    w[:, b.rows[2][3]], w[:, b.rows[2][400]] = float("inf"), float("nan")
+    w[:, b.rows[2][10]] = -1.0
+    b.weights = w
+    b.d_weights = w.cuda()
+    _evict_case(b, 450, 9)
+
+
+def test_evict_longer_than_shared_memory_holds():
+    """Past 45056 candidates the selection reads the rest of the weights again in every pass."""
+    _evict_case(Batch([1], [50000], seed=33, hkv=1, dim=64, page=64), 1200, 33)
+
+
+def test_evict_then_attend():
+    """The kept keys are attended exactly as a cache that only ever held them."""
+    b = Batch([2, 3], [200, 90], seed=34)
+    lens, kept = serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, 50, recent=8)
+    b.key_cache, b.value_cache = b.d_key.cpu(), b.d_value.cpu()
+    b.weights, b.d_seq = b.d_weights.cpu(), lens
+    b.lens = lens.tolist()
+    b.rows = [r[:c] for r, c in zip(b.rows, b.lens)]
+    for norm in NORMS:
+        b.d_weights = b.weights.cuda()
+        _chunk_case(b, norm)
+
+
+# ---------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------
+def test_gradients_are_refused():
+    b = Batch([2], [20], seed=40)
+    b.d_query.requires_grad_(True)
+    with pytest.raises(ValueError, match="inference only"):
+        b.chunk("softmax1")
+    with torch.no_grad():
+        assert torch.isfinite(b.chunk("softmax1")).all()
+
+
+def test_tensors_elsewhere_are_refused():
+    b = Batch([2], [20], seed=41)
+    with pytest.raises(ValueError, match="requires CUDA"):
+        serving.paged_chunk_attention(b.query, b.key_cache, b.value_cache, b.table, b.cu, b.seq, b.page)
+    with pytest.raises(ValueError, match="one device"):
+        serving.paged_chunk_attention(b.d_query, b.d_key, b.d_value, b.table, b.d_cu, b.d_seq, b.page)

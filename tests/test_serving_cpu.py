@@ -1,0 +1,79 @@
+"""Argument checks of the paged serving operators that need no GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+import hf_attention_normalizers_b200 as H
+from hf_attention_normalizers_b200 import _native as N
+from hf_attention_normalizers_b200 import serving
+
+
+def _args(**kw):
+    a = dict(query=torch.zeros(3, 4, 16), key_cache=torch.zeros(64, 2, 16), value_cache=torch.zeros(64, 2, 16),
+             block_table=torch.zeros(2, 2, dtype=torch.int32), cu_seqlens_q=torch.tensor([0, 1, 3], dtype=torch.int32),
+             sequence_lengths=torch.tensor([5, 9], dtype=torch.int32), block_size=16)
+    a.update(kw)
+    return a
+
+
+def test_serving_is_reached_through_the_package():
+    assert H.serving is serving and all(callable(getattr(serving, n)) for n in serving.__all__)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(), "requires CUDA tensors"),
+    (dict(key_cache=torch.zeros(64, 32)), "must have matching"),
+    (dict(value_cache=torch.zeros(64, 2, 8)), "must have matching"),
+    (dict(value_cache=torch.zeros(64, 2, 16).half()), "one dtype"),
+    (dict(value_cache=torch.zeros(64, 16, 2).transpose(1, 2)), "unit innermost stride"),
+])
+def test_cache_checks(kw, msg):
+    with pytest.raises(ValueError, match=msg):
+        serving.paged_chunk_attention(**_args(**kw))
+    a = _args(**kw)
+    with pytest.raises(ValueError, match=msg):
+        serving.paged_append(torch.zeros(3, 2, 16), torch.zeros(3, 2, 16), a["key_cache"], a["value_cache"],
+                             a["block_table"], a["cu_seqlens_q"], a["sequence_lengths"], 16)
+    with pytest.raises(ValueError, match=msg):
+        serving.paged_evict(a["key_cache"], a["value_cache"], torch.zeros(2, 64), a["block_table"], a["sequence_lengths"],
+                            16, 4)
+
+
+def _desc(**kw):
+    d = dict(dtype=N.BFLOAT16, normalizer=N.SOFTMAX1, batch=2, heads_q=4, heads_kv=2, head_dim=64, total_q=3, max_len_q=2,
+             page_size=16, max_blocks=2, max_len_k=32, num_cache_tokens=64, block_table=1, cu_seqlens_q=1, seq_lens=1,
+             scale=0.1, causal=1)
+    d.update(kw)
+    return N.ChunkDesc(**d)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(normalizer=5), "unknown normalizer"),
+    (dict(dtype=5), "unknown dtype"),
+    (dict(heads_q=5), "divisible"),
+    (dict(head_dim=257), "head_dim"),
+    (dict(batch=70000), "batch larger"),
+    (dict(page_size=0), "block_size"),
+    (dict(max_len_k=33), "enough blocks"),
+    (dict(block_table=None), "required"),
+    (dict(cu_seqlens_q=None), "cu_seqlens_q"),
+    (dict(total_q=-1), "negative"),
+    (dict(total_q=2 ** 30), "rows in one call"),
+])
+def test_requests_are_refused_on_the_host(kw, msg):
+    lib, t = N.lib(), N.HfanTensor(None, 0, 0, 0)
+    one = ctypes.c_void_p(1)
+    assert lib.hfan_paged_chunk_fwd(ctypes.byref(_desc(**kw)), t, t, t, t, one, None, 0, None) == 1
+    assert msg in lib.hfan_last_error().decode()
+    assert lib.hfan_paged_key_weights(ctypes.byref(_desc(**kw)), t, t, one, one, 64, None) == 1
+    assert lib.hfan_paged_append(ctypes.byref(_desc(**kw)), t, t, t, t, None, 0, None) == 1
+    assert lib.hfan_paged_chunk_workspace_bytes(ctypes.byref(_desc(**kw))) == -1
+
+
+@pytest.mark.parametrize("budget,recent,ld,msg", [(0, 0, 64, "budget"), (4, -1, 64, "recent"), (4, 0, 63, "every cache slot")])
+def test_evict_requests_are_refused_on_the_host(budget, recent, ld, msg):
+    lib, t, one = N.lib(), N.HfanTensor(None, 0, 0, 0), ctypes.c_void_p(1)
+    assert lib.hfan_paged_evict(ctypes.byref(_desc(cu_seqlens_q=None)), t, t, one, ld, budget, recent, one, one, None) == 1
+    assert msg in lib.hfan_last_error().decode()
