@@ -493,7 +493,7 @@ int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc) {
   AttnParams p;
   std::memset(&p, 0, sizeof(p));
   if (fill_chunk_rows(desc, p) != HFAN_OK) return -1;
-  return 0;
+  return chunk_tc_workspace(p);
 }
 
 int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, hfan_tensor value_cache,
@@ -504,7 +504,18 @@ int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor
   if (desc->total_q == 0 || desc->max_len_q == 0) return HFAN_OK;
   if (stats == nullptr) return fail(HFAN_ERR_INVALID, "stats buffer is required");
   p.stats = stats;
-  cudaError_t e = simt_attention_fwd(desc->dtype, p, desc->max_len_q, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (chunk_tc_supported(desc->dtype, p)) {
+    const int64_t need = chunk_tc_workspace(p);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+      return fail(HFAN_ERR_INVALID, "paged chunk: workspace of %lld bytes required", (long long)need);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+      return fail(HFAN_ERR_INVALID, "paged chunk: workspace must be 256-byte aligned");
+    e = chunk_tc_fwd(desc->dtype, p, workspace, s);
+  } else {
+    e = simt_attention_fwd(desc->dtype, p, desc->max_len_q, s);
+  }
   return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_chunk_fwd");
 }
 
@@ -518,7 +529,10 @@ int hfan_paged_key_weights(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tens
   if (stats == nullptr || key_weights == nullptr)
     return fail(HFAN_ERR_INVALID, "stats and key_weights buffers are required");
   p.stats = const_cast<float*>(stats);
-  cudaError_t e = serving_key_weights(desc->dtype, p, key_weights, ld_weights, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = chunk_tc_weights_supported(desc->dtype, p)
+                      ? chunk_tc_weights(desc->dtype, p, key_weights, ld_weights, s)
+                      : serving_key_weights(desc->dtype, p, key_weights, ld_weights, s);
   return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_key_weights");
 }
 

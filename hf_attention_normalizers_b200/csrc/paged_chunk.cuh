@@ -1,0 +1,91 @@
+// Shared by the tensor-core kernels of the ragged chunk attention: how packed
+// query rows and key tiles are cut, and the loads of a page-table key tile.
+//
+// The G = Hq / Hkv query heads of a KV head read the same keys, so the rows of
+// a tile are (token, head) pairs, head fastest: a tile of 128 rows holds `tpb`
+// tokens (128 / G rounded down, or fewer when no sequence brings that many)
+// and every byte of K and V serves the whole group.
+#pragma once
+
+#include "params.cuh"
+#include "tc_common.cuh"
+
+namespace hfan {
+
+constexpr int kTileRows = 128;  // packed (token, head) rows of one tile
+constexpr int kTileKeys = 128;
+
+struct ChunkPlan {
+  int group;     // query heads per KV head
+  int tpb;       // tokens per tile
+  int box_rows;  // rows of one TMA box of a page: a power of two that divides the page size, 8 .. 128
+  int splits;    // parts of the key axis (grid z)
+  int span;      // key tiles per part
+  int pairs;     // upper bound of the tile pairs of all sequences (grid x)
+};
+
+// Tokens of sequence b and the first of them, clamped as geometry() does.
+__device__ __forceinline__ int chunk_tokens(const AttnParams& p, int b, int* start) {
+  const int s = min(max(p.cu_q[b], 0), p.rows_total);
+  *start = s;
+  return min(max(p.cu_q[b + 1], s), p.rows_total) - s;
+}
+
+// The x-th group of `per` tokens over all sequences (the last of a sequence
+// may hold fewer).  Whole-warp call, uniform result; false past the last one.
+__device__ __forceinline__ bool find_group(const AttnParams& p, int per, int x, int* b, int* idx) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < p.batch; base += 32) {
+    int cnt = 0, s;
+    if (base + lane < p.batch) cnt = (chunk_tokens(p, base + lane, &s) + per - 1) / per;
+    int inc = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, inc > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      *b = base + l;
+      *idx = x - __shfl_sync(0xffffffffu, inc - cnt, l);
+      return true;
+    }
+    x -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
+// Cache row of the first key of lane's box of key tile kt (-1: no such box).
+// A page id outside the cache gives num_cache_tokens, which the tensor map
+// fills with zeros, and is recorded.
+__device__ __forceinline__ int tile_box_row(const AttnParams& p, const ChunkPlan& c, int b, int k_len, int kt) {
+  const int off = (threadIdx.x & 31) * c.box_rows, key = kt * kTileKeys + off;
+  if (off >= kTileKeys || key >= k_len) return -1;
+  const int page = p.block_table[(int64_t)b * p.max_blocks + key / p.page_size];
+  const int64_t row = (int64_t)page * p.page_size + key % p.page_size;
+  if (page < 0 || row >= p.num_cache_tokens) {
+    if (p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevBadPage);
+    return (int)p.num_cache_tokens;
+  }
+  return (int)row;
+}
+
+// Loads the boxes of one key tile (rows from tile_box_row) into a stage of
+// NH swizzled halves.  Whole-warp call; rows of keys past k_len in the last
+// box hold whatever the page holds, boxes past it keep the stage's old bytes.
+template <int NH>
+__device__ __forceinline__ void load_key_tile_tma(uint8_t* stage, const CUtensorMap* map, uint64_t* bar, int row,
+                                                  int box_rows, int kvh) {
+  const unsigned have = __ballot_sync(0xffffffffu, row >= 0);
+  if ((threadIdx.x & 31) == 0)
+    tc::mbar_arrive_expect_tx(bar, (uint32_t)__popc(have) * (uint32_t)box_rows * 128u * NH);
+  __syncwarp();
+  if (row >= 0) {
+    uint8_t* dst = stage + (threadIdx.x & 31) * box_rows * 128;
+#pragma unroll
+    for (int hh = 0; hh < NH; ++hh) tc::tma_load_4d(dst + hh * tc::kHalf, map, bar, 64 * hh, row, kvh, 0);
+  }
+}
+
+}  // namespace hfan

@@ -1,0 +1,769 @@
+// Attention of a ragged chunk of new tokens over a paged cache, on tcgen05
+// tensor cores (16-bit inputs, head_dim 64 / 128, pages of a multiple of 8
+// tokens, positive scale).
+//
+// One CTA takes two tiles of 128 packed (token, head) rows of one sequence and
+// KV head over one part of its keys, in tiles of 128 keys that TMA fetches
+// straight from the pages (one box per page or per 128 rows of it):
+//
+//   warps 0-3, 4-7  row warps of tile 0 / 1: thread = TMEM lane = row.  A
+//                   thread reads its whole S row, so the running maximum and
+//                   sum need no exchange, and writes P over S as packed
+//                   16-bit pairs (the A operand of P V).
+//   warp 8          producer: Q once, then K0 V0 K1 V1 ... through one ring.
+//   warps 9, 10     MMA issuers of tile 0 / 1: S = Q K^T, then O += P V, then
+//                   the next S over the P just consumed.
+//
+// The two tiles are independent chains that share the K and V stages: while
+// one chain's row warps exponentiate, the tensor pipe works for the other.
+// softmax1 keeps a reference m >= 0 (the implicit zero logit) that follows the
+// row maximum lazily: O is rescaled only when the maximum grew by more than
+// 2^8.  P V of tile t is done before S of tile t + 1 (same issuer), so the row
+// warps that hold S of t + 1 may rescale O without another wait.
+//
+// With few rows the key axis is split over grid z; the parts leave unscaled O
+// with (m, l) in the workspace and combine_kernel joins them.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "paged_chunk.cuh"
+#include "paged_serving.cuh"
+#include "params.cuh"
+#include "tc_common.cuh"
+#include "tc_ptx.cuh"
+
+namespace hfan {
+namespace {
+
+using namespace tc;
+
+constexpr int kChunkThreads = 384;
+// Registers of a thread: 384 x 168 at launch; the helper warpgroup (producer,
+// issuers) gives up what lets a row thread hold its S row without spills.
+constexpr int kRowRegs = 224, kHelperRegs = 56;
+static_assert(256 * kRowRegs + 128 * kHelperRegs <= 384 * 168, "more registers than the block was launched with");
+constexpr int kMaxRing = 8;
+constexpr float kRescale = 8.f;
+
+template <int HD>
+constexpr int chunk_ring() { return HD == 128 ? 5 : 8; }
+
+struct ChunkBars {
+  uint64_t q_full, full[kMaxRing], empty[kMaxRing];
+  uint64_t s_full[2], p_full[2], o_full[2], drain[2];
+};
+struct ChunkCtl {
+  uint32_t tmem;
+  int abort, never;  // never stays 0: the abort flag of waits that must not be cut short
+};
+
+template <int HD>
+struct ChunkLayout {
+  static constexpr int NH = HD / 64, NS = chunk_ring<HD>();
+  static constexpr uint32_t TILE = NH * kHalf;
+  static constexpr uint32_t RING = 2 * TILE;
+  static constexpr uint32_t BARS = RING + NS * TILE;
+  static constexpr uint32_t CTL = BARS + sizeof(ChunkBars);
+  static constexpr uint32_t TOTAL = CTL + sizeof(ChunkCtl) + 1024;
+};
+
+// Partial results of the split key axis.
+struct ChunkWs {
+  float* o;    // [splits][total_q * hq][D]
+  float2* ml;  // [splits][total_q * hq]
+  int* parts;  // [total_q * hq] parts that the row has (1: already final)
+};
+
+__device__ __forceinline__ void fail(const AttnParams& p, ChunkCtl* ctl) {
+  ctl->abort = 1;
+  if (p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevWaitTimeout);
+}
+
+template <int HD, bool BF16, int NORM>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    chunk_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const AttnParams p, const ChunkPlan c, const ChunkWs ws) {
+  using L = ChunkLayout<HD>;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int NH = L::NH, NS = L::NS;
+  constexpr uint32_t IDESC_QK = idesc_f16(BF16, 128, 128, false, false);
+  constexpr uint32_t IDESC_PV = idesc_f16(BF16, 128, HD, false, true);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  ChunkBars* bars = reinterpret_cast<ChunkBars*>(smem + L::BARS);
+  ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(smem + L::CTL);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  int b, pair;
+  if (!find_group(p, 2 * c.tpb, blockIdx.x, &b, &pair)) return;
+  const Geometry g = geometry(p, b);
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int tok0 = pair * 2 * c.tpb, ntok = min(2 * c.tpb, g.q_len - tok0);
+  const int nact = ntok > c.tpb ? 2 : 1;  // tiles with rows
+  const int k_hi = p.causal ? min(g.k_len, tok0 + ntok + g.shift) : g.k_len;
+  const int n_all = k_hi > 0 ? (k_hi + kTileKeys - 1) / kTileKeys : 0;
+  const int parts = max(1, (n_all + c.span - 1) / c.span);
+  if (split >= parts) return;
+  const int kt0 = split * c.span, nt = min(c.span, n_all - kt0);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], nact);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], 4);
+      mbar_init(&bars->o_full[s], 1);
+      mbar_init(&bars->drain[s], 1);
+    }
+    ctl->abort = ctl->never = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(&ctl->tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;  // S0 | S1 | O0 | O1, 128 columns each
+  volatile int* abort_flag = &ctl->abort;
+
+  if (warp >= 8) {
+  set_max_regs<kHelperRegs, false>();
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (nt > 0) {
+      if (lane == 0) {
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        mbar_arrive_expect_tx(&bars->q_full, nact * NH * c.tpb * c.group * 128);
+        for (int q = 0; q < nact; ++q)
+          for (int hh = 0; hh < NH; ++hh)
+            tma_load_4d(smem + q * L::TILE + hh * kHalf, &tm_q, &bars->q_full, 64 * hh, kvh * c.group,
+                        g.q_start + tok0 + q * c.tpb, 0);
+      }
+      bool ok = true;
+      int row = tile_box_row(p, c, b, g.k_len, kt0);
+      int st = 0, ph = 1;
+      int issued = 0;
+      for (int t = 0; t < nt && ok; ++t) {
+        const int next = t + 1 < nt ? tile_box_row(p, c, b, g.k_len, kt0 + t + 1) : -1;
+#pragma unroll
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          if (!(ok = wait_warp(&bars->empty[st], ph, abort_flag))) break;
+          load_key_tile_tma<NH>(smem + L::RING + st * L::TILE, kv ? &tm_v : &tm_k, &bars->full[st], row, c.box_rows, kvh);
+          ++issued;
+          if (++st == NS) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+        row = next;
+      }
+      if (!ok) {
+        if (lane == 0) {
+          fail(p, ctl);
+          // its own copies land before the CTA leaves
+          mbar_wait(&bars->q_full, 0, &ctl->never);
+          for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&bars->full[i % NS], (i / NS) & 1, &ctl->never);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 11) {  // (warp 11 fills the warpgroup)
+    // ------------------------------------------------------------ MMA issuers
+    const int q = warp - 9;
+    if (lane == 0 && q < nact && nt > 0) {
+      const uint32_t q_base = smem_u32(smem + q * L::TILE), ring = smem_u32(smem + L::RING);
+      const uint32_t s_col = tmem + q * 128, o_col = tmem + 256 + q * 128;
+      bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
+      int st = 0, ph = 0;
+      auto step = [&]() {
+        if (++st == NS) {
+          st = 0;
+          ph ^= 1;
+        }
+      };
+      for (int t = 0; t < nt && ok; ++t) {
+        if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+          mma_f16_ss(s_col, sw128_desc(q_base + o, 16, 1024), sw128_desc(ring + st * L::TILE + o, 16, 1024), IDESC_QK,
+                     kk > 0);
+        }
+        mma_commit(&bars->s_full[q]);
+        mma_commit(&bars->empty[st]);
+        step();
+        if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+        if (!(ok = mbar_wait(&bars->p_full[q], t & 1, abort_flag))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kTileKeys / 16; ++kk)
+          mma_f16_ts(o_col, s_col + kk * 8, sw128_desc(ring + st * L::TILE + kk * 16 * 128, kHalf, 1024), IDESC_PV,
+                     t > 0 || kk > 0);
+        mma_commit(&bars->empty[st]);
+        if (t + 1 == nt) mma_commit(&bars->o_full[q]);
+        step();
+      }
+      if (!ok) {
+        fail(p, ctl);
+        mma_commit(&bars->drain[q]);
+        mbar_wait(&bars->drain[q], 0, &ctl->never);
+      }
+    }
+    __syncwarp();
+  }
+  } else if ((warp >> 2) < nact) {
+    // ------------------------------------------------------------ row warps
+    set_max_regs<kRowRegs, true>();
+    const int q = warp >> 2, r = threadIdx.x & 127;
+    const int i = tok0 + q * c.tpb + r / c.group;  // token within the sequence
+    const bool row_ok = r < c.tpb * c.group && i < g.q_len;
+    const int h = kvh * c.group + r % c.group;
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lane_addr + q * 128, o_col = tmem + lane_addr + 256 + q * 128;
+    // visible keys [0, vis)
+    int vis = row_ok ? g.k_len : 0;
+    if (p.causal && row_ok) vis = min(vis, i + g.shift + 1);
+    const bool warp_on = __any_sync(0xffffffffu, vis > 0);
+    const float zs = NORM == HFAN_SOFTMAX1 ? p.scale * kLog2e : (NORM == HFAN_SPARSEMAX ? p.scale : 0.5f * p.scale);
+    const int64_t si = row_ok ? stat_index(p, g, h, i) : 0;
+    const int64_t srow = (int64_t)(g.q_start + i) * p.hq + h;
+    float m = 0.f, l = 0.f;
+    if (NORM != HFAN_SOFTMAX1) m = row_ok ? p.stats[si] : kPosInf;  // the threshold
+    bool ok = true;
+    int vst = 1 % NS, vph = 0;  // stage of V
+    for (int t = 0; t < nt; ++t) {
+      if (!(ok = wait_warp(&bars->s_full[q], t & 1, abort_flag))) break;
+      tc_fence_after();
+      const int kb = (kt0 + t) * kTileKeys;
+      if (kb + kTileKeys > g.k_len) {
+        // V rows past the sequence hold stale or foreign values: zeroed, since
+        // 0 x NaN would reach O (both tiles' warps write the same zeros)
+        if (!(ok = wait_warp(&bars->full[vst], vph, abort_flag))) break;
+        const int lo = g.k_len - kb;
+        uint8_t* v = smem + L::RING + vst * L::TILE;
+        for (int x = r; x < (kTileKeys - lo) * 8 * NH; x += 128) {
+          const int hh = x / ((kTileKeys - lo) * 8), y = x - hh * (kTileKeys - lo) * 8;
+          *reinterpret_cast<uint4*>(v + hh * kHalf + lo * 128 + y * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      vst += 2;
+      if (vst >= NS) {
+        vst -= NS;
+        vph ^= 1;
+      }
+      uint32_t pk[64];
+      if (warp_on) {
+        float s[128];
+        {
+          uint32_t x[4][32];
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) tmem_ld32(s_col + cc * 32, x[cc]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 128; ++j) s[j] = __uint_as_float(x[j >> 5][j & 31]);
+        }
+        const int lim = vis - kb;
+        if (!__all_sync(0xffffffffu, lim >= kTileKeys)) {
+#pragma unroll
+          for (int j = 0; j < 128; ++j) s[j] = j < lim ? s[j] : kNegInf;
+        }
+        const uint64_t zs2 = f2_pack(zs, zs);
+        if (NORM == HFAN_SOFTMAX1) {
+          const float top = max_n<128>(s) * zs;
+          float alpha = 1.f;
+          if (top > m + kRescale) {
+            alpha = exp2f(m - top);
+            m = top;
+            l *= alpha;
+          }
+          if (__any_sync(0xffffffffu, alpha != 1.f) && t > 0) {
+#pragma unroll
+            for (int cc = 0; cc < HD / 32; ++cc) {
+              uint32_t o[32];
+              tmem_ld32(o_col + cc * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st32(o_col + cc * 32, o);
+            }
+          }
+          const uint64_t nm2 = f2_pack(-m, -m);
+          uint64_t l2 = 0;
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) {
+            const uint64_t x = ffma2(f2_pack(s[j], s[j + 1]), zs2, nm2);
+            const float e0 = ex2_ftz(f2_lo(x)), e1 = ex2_ftz(f2_hi(x));
+            l2 = fadd2(l2, f2_pack(e0, e1));
+            pk[j / 2] = pack2<BF16>(e0, e1);
+          }
+          l += f2_lo(l2) + f2_hi(l2);
+        } else {
+          const uint64_t nt2 = f2_pack(-m, -m);
+#pragma unroll
+          for (int j = 0; j < 128; j += 2) {
+            const uint64_t x = ffma2(f2_pack(s[j], s[j + 1]), zs2, nt2);
+            uint64_t d = f2_pack(fmaxf(f2_lo(x), 0.f), fmaxf(f2_hi(x), 0.f));
+            if (NORM == HFAN_ENTMAX15) d = fmul2(d, d);
+            pk[j / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) pk[j] = 0u;
+      }
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc) tmem_st32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(pk + cc * 32));
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(&bars->p_full[q]);
+    }
+    if (ok && nt > 0) ok = wait_warp(&bars->o_full[q], 0, abort_flag);
+    tc_fence_after();
+    if (!ok && lane == 0) fail(p, ctl);
+    const bool last = parts == 1;
+    if (NORM == HFAN_SOFTMAX1 && last) l += exp2f(-m);  // the implicit zero logit
+    const float inv = NORM == HFAN_SOFTMAX1 && last ? 1.f / l : 1.f;
+    if (warp_on || last) {
+#pragma unroll
+      for (int cc = 0; cc < HD / 32; ++cc) {
+        uint32_t o[32];
+        if (nt > 0 && ok) {
+          tmem_ld32(o_col + cc * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        if (!row_ok) continue;
+        if (last) {
+          T* dst = static_cast<T*>(p.o) + (int64_t)(g.q_start + i) * p.o_st + (int64_t)h * p.o_sh + cc * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 v;
+            v.x = pack2<BF16>(__uint_as_float(o[j + 0]) * inv, __uint_as_float(o[j + 1]) * inv);
+            v.y = pack2<BF16>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+            v.z = pack2<BF16>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
+            v.w = pack2<BF16>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + j) = v;
+          }
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(ws.o + ((int64_t)split * p.rows_total * p.hq + srow) * HD + cc * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+      }
+    }
+    if (row_ok) {
+      if (last && NORM == HFAN_SOFTMAX1) {
+        p.stats[si] = m;
+        p.stats[(int64_t)p.hq * p.rows_total + si] = l;
+      }
+      if (!last && NORM == HFAN_SOFTMAX1) ws.ml[(int64_t)split * p.rows_total * p.hq + srow] = make_float2(m, l);
+      if (split == 0 && ws.parts != nullptr) ws.parts[srow] = parts;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of a row: one warp per (token, head).
+template <int HD, typename T, int NORM>
+__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p, const ChunkWs ws, int splits) {
+  const int64_t rows = (int64_t)p.rows_total * p.hq, row = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int parts = min(ws.parts[row], splits);  // (a row that no sequence owns has none)
+  if (parts < 2) return;
+  const int tok = (int)(row / p.hq), h = (int)(row - (int64_t)tok * p.hq);
+  constexpr int N = HD / 32;
+  float m = 0.f, l = 0.f;
+  if (NORM == HFAN_SOFTMAX1) {
+    for (int s = lane; s < parts; s += 32) m = fmaxf(m, ws.ml[s * rows + row].x);
+    m = warp_max(m);
+    for (int s = lane; s < parts; s += 32) {
+      const float2 x = ws.ml[s * rows + row];
+      l += x.y * exp2f(x.x - m);
+    }
+    l = warp_sum(l) + exp2f(-m);
+  }
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float f = NORM == HFAN_SOFTMAX1 ? exp2f(ws.ml[s * rows + row].x - m) : 1.f;
+    const float* o = ws.o + (s * rows + row) * HD + lane * N;
+    if constexpr (N == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(o);
+      acc[0] = fmaf(f, x.x, acc[0]);
+      acc[1] = fmaf(f, x.y, acc[1]);
+      acc[2] = fmaf(f, x.z, acc[2]);
+      acc[3] = fmaf(f, x.w, acc[3]);
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(o);
+      acc[0] = fmaf(f, x.x, acc[0]);
+      acc[1] = fmaf(f, x.y, acc[1]);
+    }
+  }
+  const float inv = NORM == HFAN_SOFTMAX1 ? 1.f / l : 1.f;
+  T* dst = static_cast<T*>(p.o) + (int64_t)tok * p.o_st + (int64_t)h * p.o_sh + lane * N;
+#pragma unroll
+  for (int e = 0; e < N; ++e) dst[e] = from_f32<T>(acc[e] * inv);
+  if (NORM == HFAN_SOFTMAX1 && lane == 0) {
+    p.stats[(int64_t)h * p.rows_total + tok] = m;
+    p.stats[(int64_t)p.hq * p.rows_total + (int64_t)h * p.rows_total + tok] = l;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Key weights: w[key] = sum over the chunk's packed rows of p(row, key), from
+// the rows' statistics.  The scores are taken transposed, S^T = K Q^T, so that
+// a thread owns a key and sums over the columns without any exchange: one CTA
+// takes 128 keys of one (sequence, KV head) and walks the row tiles, its two
+// warpgroups alternating between them.  No reference to the maximum is
+// needed: p = 2^(s zs - (m + log2 l)) (softmax1) or (s zs - tau)_+^a.
+// ---------------------------------------------------------------------------
+struct WeightBars {
+  uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2], drain[2];
+};
+template <int HD>
+struct WeightLayout {
+  static constexpr int NH = HD / 64;
+  static constexpr uint32_t TILE = NH * kHalf;
+  static constexpr uint32_t Q = TILE;
+  static constexpr uint32_t CONSTS = Q + 2 * TILE;  // [2][128] row constants
+  static constexpr uint32_t SUMS = CONSTS + 2 * 128 * 4;
+  static constexpr uint32_t BARS = SUMS + 128 * 4;
+  static constexpr uint32_t CTL = BARS + sizeof(WeightBars);
+  static constexpr uint32_t TOTAL = CTL + sizeof(ChunkCtl) + 1024;
+};
+
+constexpr int kWeightThreads = 352;
+
+template <int HD, bool BF16, int NORM>
+__global__ void __launch_bounds__(kWeightThreads, 2)
+    chunk_weights_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const AttnParams p, const ChunkPlan c, float* kw, int64_t ldw) {
+  using L = WeightLayout<HD>;
+  constexpr int NH = L::NH;
+  const int b = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * kTileKeys;
+  const Geometry g = geometry(p, b);
+  if (k0 >= g.k_len || g.q_len == 0) return;
+  // row tiles that see the first key of this key tile
+  const int i_lo = p.causal ? max(0, k0 - g.shift) : 0;
+  const int t_lo = i_lo / c.tpb, t_hi = (g.q_len + c.tpb - 1) / c.tpb;
+  if (t_lo >= t_hi) return;
+  const int nt = t_hi - t_lo;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  WeightBars* bars = reinterpret_cast<WeightBars*>(smem + L::BARS);
+  ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(smem + L::CTL);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->k_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->q_full[s], 1);
+      mbar_init(&bars->q_empty[s], 1);
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->s_empty[s], 4);
+      mbar_init(&bars->drain[s], 1);
+    }
+    ctl->abort = ctl->never = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(&ctl->tmem, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;  // S^T of warpgroup 0 | 1
+  volatile int* abort_flag = &ctl->abort;
+  // packed rows of row tile t, and the MMA's N (a multiple of 16) that covers them
+  auto rows_of = [&](int t) { return min(c.tpb, g.q_len - t * c.tpb) * c.group; };
+
+  if (warp == 8) {
+    load_key_tile_tma<NH>(smem, &tm_k, &bars->k_full, tile_box_row(p, c, b, g.k_len, blockIdx.x), c.box_rows, kvh);
+    if (lane == 0) {
+      bool ok = true;
+      int u = 0;
+      for (; u < nt && ok; ++u) {
+        const int st = u & 1;
+        if (!(ok = mbar_wait(&bars->q_empty[st], ((u >> 1) & 1) ^ 1, abort_flag))) break;
+        mbar_arrive_expect_tx(&bars->q_full[st], NH * c.tpb * c.group * 128);
+        for (int hh = 0; hh < NH; ++hh)
+          tma_load_4d(smem + L::Q + st * L::TILE + hh * kHalf, &tm_q, &bars->q_full[st], 64 * hh, kvh * c.group,
+                      g.q_start + (t_lo + u) * c.tpb, 0);
+      }
+      if (!ok) {
+        fail(p, ctl);
+        mbar_wait(&bars->k_full, 0, &ctl->never);
+        for (int i = max(0, u - 2); i < u; ++i) mbar_wait(&bars->q_full[i & 1], (i >> 1) & 1, &ctl->never);
+      }
+    }
+    __syncwarp();
+  } else if (warp > 8) {
+    const int w = warp - 9;
+    if (lane == 0 && w < nt) {
+      const uint32_t k_base = smem_u32(smem), q_base = smem_u32(smem + L::Q + w * L::TILE);
+      bool ok = mbar_wait(&bars->k_full, 0, abort_flag);
+      for (int u = w; u < nt && ok; u += 2) {
+        const int ph = (u >> 1) & 1;
+        if (!(ok = mbar_wait(&bars->q_full[w], ph, abort_flag))) break;
+        if (!(ok = mbar_wait(&bars->s_empty[w], ph ^ 1, abort_flag))) break;
+        tc_fence_after();
+        const uint32_t idesc = idesc_f16(BF16, 128, (rows_of(t_lo + u) + 15) & ~15, false, false);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+          mma_f16_ss(tmem + w * 128, sw128_desc(k_base + o, 16, 1024), sw128_desc(q_base + o, 16, 1024), idesc, kk > 0);
+        }
+        mma_commit(&bars->s_full[w]);
+        mma_commit(&bars->q_empty[w]);
+      }
+      if (!ok) {
+        fail(p, ctl);
+        mma_commit(&bars->drain[w]);
+        mbar_wait(&bars->drain[w], 0, &ctl->never);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int w = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t s_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + w * 128;
+    float* consts = reinterpret_cast<float*>(smem + L::CONSTS) + w * 128;
+    const float zs = NORM == HFAN_SOFTMAX1 ? p.scale * kLog2e : (NORM == HFAN_SPARSEMAX ? p.scale : 0.5f * p.scale);
+    const uint64_t zs2 = f2_pack(zs, zs);
+    const int key = k0 + r;
+    float total = 0.f;
+    bool ok = true;
+    for (int u = w; u < nt; u += 2) {
+      const int t = t_lo + u, nrows = rows_of(t);
+      float cst = 0.f;
+      if (r < nrows) {
+        const int64_t si = stat_index(p, g, kvh * c.group + r % c.group, t * c.tpb + r / c.group);
+        const float s0 = p.stats[si];
+        cst = NORM == HFAN_SOFTMAX1 ? -(s0 + log2f(p.stats[(int64_t)p.hq * p.rows_total + si])) : -s0;
+      }
+      named_bar_sync(1 + w, 128);  // the previous tile's constants have been read
+      consts[r] = cst;
+      named_bar_sync(1 + w, 128);
+      if (ok) ok = wait_warp(&bars->s_full[w], (u >> 1) & 1, abort_flag);
+      if (!ok) continue;  // the warpgroup keeps meeting at its barrier
+      tc_fence_after();
+      // rows [lo, nrows) see this thread's key
+      int lo = 0;
+      if (p.causal) lo = max(0, (key - g.shift - t * c.tpb)) * c.group;
+      const bool full = __all_sync(0xffffffffu, lo == 0 && nrows == 128);
+      uint64_t sum2 = 0;
+      for (int cc = 0; cc * 32 < nrows; ++cc) {
+        uint32_t x[32];
+        tmem_ld32(s_col + cc * 32, x);
+        tmem_wait_ld();
+        const float4* c4 = reinterpret_cast<const float4*>(consts + cc * 32);
+        if (!full) {
+          // scores of rows that are not there may be anything
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = cc * 32 + j >= lo && cc * 32 + j < nrows ? x[j] : 0xff800000u;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 k4 = c4[j / 4];
+          uint64_t a = ffma2(f2_pack(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), zs2, f2_pack(k4.x, k4.y));
+          uint64_t e = ffma2(f2_pack(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), zs2, f2_pack(k4.z, k4.w));
+          if (NORM == HFAN_SOFTMAX1) {
+            a = f2_pack(ex2_ftz(f2_lo(a)), ex2_ftz(f2_hi(a)));
+            e = f2_pack(ex2_ftz(f2_lo(e)), ex2_ftz(f2_hi(e)));
+          } else {
+            a = f2_pack(fmaxf(f2_lo(a), 0.f), fmaxf(f2_hi(a), 0.f));
+            e = f2_pack(fmaxf(f2_lo(e), 0.f), fmaxf(f2_hi(e), 0.f));
+            if (NORM == HFAN_ENTMAX15) {
+              a = fmul2(a, a);
+              e = fmul2(e, e);
+            }
+          }
+          sum2 = fadd2(sum2, fadd2(a, e));
+        }
+      }
+      total += f2_lo(sum2) + f2_hi(sum2);
+      tc_fence_before();
+      warp_arrive(&bars->s_empty[w]);
+    }
+    if (!ok && lane == 0) fail(p, ctl);
+    float* sums = reinterpret_cast<float*>(smem + L::SUMS);
+    if (w == 1) sums[r] = total;
+    named_bar_sync(3, 256);
+    if (w == 0 && key < g.k_len) {
+      total += sums[r];
+      const int64_t tok = key_token(p, g, b, key);
+      if (tok >= 0) atomicAdd(kw + (int64_t)kvh * ldw + tok, total);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// ------------------------------------------------------------------ host
+int pow2_divisor(int n, int most) {
+  int r = 1;
+  while (r < most && n % (2 * r) == 0) r *= 2;
+  return r;
+}
+
+int sm_count() {
+  static int n[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n[dev];
+}
+
+ChunkPlan plan_of(const AttnParams& p) {
+  ChunkPlan c;
+  c.group = p.hq / p.hkv;
+  const int most = c.group < kTileRows ? kTileRows / c.group : 1;  // (larger groups run on the general kernels)
+  const int longest = p.len_q < p.rows_total ? p.len_q : p.rows_total;
+  c.tpb = longest < most ? (longest > 0 ? longest : 1) : most;
+  c.box_rows = pow2_divisor(p.page_size, kTileKeys);
+  // every sequence may leave one part-filled pair
+  const int64_t pairs = p.rows_total / (2 * c.tpb) + (p.batch < p.rows_total ? p.batch : p.rows_total);
+  c.pairs = (int)(pairs < 1 ? 1 : pairs);
+  const int ktiles = (p.len_k + kTileKeys - 1) / kTileKeys;
+  // One wave of CTAs over the SMs; a part shorter than four key tiles would
+  // pay more for its prologue and its partial result than it saves.
+  const int64_t units = (int64_t)c.pairs * p.hkv;
+  int64_t splits = units > 0 ? sm_count() / units : 1;
+  if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
+  if (splits < 1) splits = 1;
+  c.span = (int)((ktiles + splits - 1) / splits);
+  if (c.span < 1) c.span = 1;
+  c.splits = (ktiles + c.span - 1) / c.span;
+  if (c.splits < 1) c.splits = 1;
+  return c;
+}
+
+struct WsLayout {
+  int64_t o, ml, parts, total;
+};
+WsLayout ws_layout(const AttnParams& p, const ChunkPlan& c) {
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  const int64_t rows = (int64_t)p.rows_total * p.hq;
+  WsLayout w{0, 0, 0, 0};
+  if (c.splits < 2) return w;
+  w.ml = up(rows * c.splits * p.d * 4);
+  w.parts = w.ml + up(rows * c.splits * 8);
+  w.total = w.parts + up(rows * 4);
+  return w;
+}
+
+// (dim, head, token) map of packed rows: a box is one tile, rows token-major.
+bool make_row_map(CUtensorMap* m, const AttnParams& p, bool bf16, const ChunkPlan& c) {
+  return make_map_box(m, p.q, bf16, {(cuuint64_t)p.d, (cuuint64_t)p.hq, (cuuint64_t)p.rows_total, 1},
+                      {p.q_sh, p.q_st, p.q_st * p.rows_total}, {64, (cuuint32_t)c.group, (cuuint32_t)c.tpb, 1});
+}
+bool make_page_map(CUtensorMap* m, const void* cache, int64_t st, int64_t sh, const AttnParams& p, bool bf16,
+                   const ChunkPlan& c) {
+  return make_map(m, cache, bf16, p.d, p.num_cache_tokens, p.hkv, 1, st, sh, p.num_cache_tokens * st, c.box_rows);
+}
+
+template <int HD, bool BF16, int NORM>
+cudaError_t fwd_t(const AttnParams& p, const ChunkPlan& c, void* workspace, cudaStream_t s) {
+  CUtensorMap tq, tk, tv;
+  if (!make_row_map(&tq, p, BF16, c) || !make_page_map(&tk, p.k, p.k_st, p.k_sh, p, BF16, c) ||
+      !make_page_map(&tv, p.v, p.v_st, p.v_sh, p, BF16, c))
+    return cudaErrorInvalidValue;
+  const WsLayout w = ws_layout(p, c);
+  ChunkWs ws{nullptr, nullptr, nullptr};
+  if (c.splits > 1) {
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    ws.o = reinterpret_cast<float*>(base + w.o);
+    ws.ml = reinterpret_cast<float2*>(base + w.ml);
+    ws.parts = reinterpret_cast<int*>(base + w.parts);
+  }
+  auto kernel = chunk_fwd_kernel<HD, BF16, NORM>;
+  constexpr int smem = ChunkLayout<HD>::TOTAL;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3(c.pairs, p.hkv, c.splits), kChunkThreads, smem, s>>>(tq, tk, tv, p, c, ws);
+  if (c.splits > 1) {
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    const int64_t rows = (int64_t)p.rows_total * p.hq;
+    combine_kernel<HD, T, NORM><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p, ws, c.splits);
+  }
+  return cudaGetLastError();
+}
+
+template <int HD, bool BF16, int NORM>
+cudaError_t weights_t(const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw, cudaStream_t s) {
+  CUtensorMap tq, tk;
+  if (!make_row_map(&tq, p, BF16, c) || !make_page_map(&tk, p.k, p.k_st, p.k_sh, p, BF16, c))
+    return cudaErrorInvalidValue;
+  auto kernel = chunk_weights_kernel<HD, BF16, NORM>;
+  constexpr int smem = WeightLayout<HD>::TOTAL;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3((p.len_k + kTileKeys - 1) / kTileKeys, p.hkv, p.batch), kWeightThreads, smem, s>>>(tq, tk, p, c, kw, ldw);
+  return cudaGetLastError();
+}
+
+// F<HD, BF16, NORM>::run(args...) for the request's types.
+#define HFAN_CHUNK_DISPATCH(fn, ...)                                                                             \
+  const bool bf16 = dtype == HFAN_BFLOAT16;                                                                      \
+  switch (p.norm) {                                                                                              \
+    case HFAN_SOFTMAX1:                                                                                          \
+      return p.d == 128 ? (bf16 ? fn<128, true, HFAN_SOFTMAX1>(__VA_ARGS__) : fn<128, false, HFAN_SOFTMAX1>(__VA_ARGS__)) \
+                        : (bf16 ? fn<64, true, HFAN_SOFTMAX1>(__VA_ARGS__) : fn<64, false, HFAN_SOFTMAX1>(__VA_ARGS__)); \
+    case HFAN_SPARSEMAX:                                                                                         \
+      return p.d == 128 ? (bf16 ? fn<128, true, HFAN_SPARSEMAX>(__VA_ARGS__) : fn<128, false, HFAN_SPARSEMAX>(__VA_ARGS__)) \
+                        : (bf16 ? fn<64, true, HFAN_SPARSEMAX>(__VA_ARGS__) : fn<64, false, HFAN_SPARSEMAX>(__VA_ARGS__)); \
+    default:                                                                                                     \
+      return p.d == 128 ? (bf16 ? fn<128, true, HFAN_ENTMAX15>(__VA_ARGS__) : fn<128, false, HFAN_ENTMAX15>(__VA_ARGS__)) \
+                        : (bf16 ? fn<64, true, HFAN_ENTMAX15>(__VA_ARGS__) : fn<64, false, HFAN_ENTMAX15>(__VA_ARGS__)); \
+  }
+
+bool keys_supported(int dtype, const AttnParams& p) {
+  if (dtype != HFAN_BFLOAT16 && dtype != HFAN_FLOAT16) return false;
+  if (p.d != 64 && p.d != 128) return false;
+  // a swizzle atom is 8 rows of a page; masked scores are -inf before the scaling
+  if (p.page_size % 8 != 0 || !(p.scale > 0.f) || p.hq / p.hkv > kTileRows) return false;
+  if (p.num_cache_tokens < 1 || p.num_cache_tokens > 0x7fffffffll) return false;
+  return aligned16(p.q) && aligned16(p.k) && stride_ok(p.q_st) && stride_ok(p.q_sh) && stride_ok(p.k_st) &&
+         stride_ok(p.k_sh);
+}
+
+}  // namespace
+
+bool chunk_tc_supported(int dtype, const AttnParams& p) {
+  return p.norm == HFAN_SOFTMAX1 && keys_supported(dtype, p) && aligned16(p.v) && aligned16(p.o) && stride_ok(p.v_st) &&
+         stride_ok(p.v_sh) && p.o_st % 8 == 0 && p.o_sh % 8 == 0;
+}
+
+int64_t chunk_tc_workspace(const AttnParams& p) { return ws_layout(p, plan_of(p)).total; }
+
+cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, void* workspace, cudaStream_t s) {
+  const ChunkPlan c = plan_of(p);
+  HFAN_CHUNK_DISPATCH(fwd_t, p, c, workspace, s)
+}
+
+bool chunk_tc_weights_supported(int dtype, const AttnParams& p) { return keys_supported(dtype, p); }
+
+cudaError_t chunk_tc_weights(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s) {
+  const ChunkPlan c = plan_of(p);
+  HFAN_CHUNK_DISPATCH(weights_t, p, c, kw, ldw, s)
+}
+
+}  // namespace hfan

@@ -150,24 +150,32 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// 4-D map (dim, token, head, batch) with a 64 x 128 x 1 x 1 box, 128-byte swizzle.
-inline bool make_map(CUtensorMap* m, const void* base, bool bf16, int d, int64_t tokens, int heads, int batch,
-              int64_t st, int64_t sh, int64_t sb, int box_rows = 128) {
+// 4-D map of 16-bit elements with a 128-byte swizzle: dims[0] is contiguous,
+// strides[i] (elements) belongs to dims[i + 1].
+inline bool make_map_box(CUtensorMap* m, const void* base, bool bf16, const cuuint64_t (&dims)[4],
+                         const int64_t (&st)[3], const cuuint32_t (&box)[4]) {
   auto fn = encode_fn();
   if (fn == nullptr) return false;
   // The encoder is a driver call and needs a current context.  A thread that
   // has made no runtime call yet (for example autograd's backward worker, when
-  // nothing ran on it before this library) has none: cudaFree(nullptr) binds
-  // the current device's primary context and does nothing else.
-  cudaFree(nullptr);
-  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
-  cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  // nothing ran on it before this library) has none: cudaSetDevice binds the
+  // device's primary context and, unlike cudaFree(nullptr), may be called
+  // while a stream is being captured.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+  cuuint64_t strides[3] = {(cuuint64_t)st[0] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
+}
+
+// 4-D map (dim, token, head, batch) with a 64 x 128 x 1 x 1 box, 128-byte swizzle.
+inline bool make_map(CUtensorMap* m, const void* base, bool bf16, int d, int64_t tokens, int heads, int batch,
+              int64_t st, int64_t sh, int64_t sb, int box_rows = 128) {
+  return make_map_box(m, base, bf16, {(cuuint64_t)d, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch},
+                      {st, sh, sb}, {64, (cuuint32_t)box_rows, 1, 1});
 }
 
 inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }

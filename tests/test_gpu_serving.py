@@ -5,8 +5,8 @@ Tolerances, from the formulas:
   * a score s = scale q.k is a float32 sum of D exact products: the error of such a sum
     is about sqrt(D) roundings of its largest partial sum, so |ds| <= DS =
     4 sqrt(D) 2^-24 scale max sum|q_d k_d|;
-  * outputs: p is rounded to the 16-bit type before P V (relative U = 2^-9 for bfloat16,
-    2^-12 for float16, 0 for float32) and so is the result; a score error moves p by at most
+  * outputs: p is rounded to the 16-bit type before P V (relative U = the type's unit
+    roundoff: 2^-8 for bfloat16, 2^-11 for float16, 2^-24 for float32) and so is the result; a score error moves p by at most
     2 DS dp/ds.  |do| <= 2 U sum p|v| + 2 DS sum g |v| + 1e-6 max|v|;
   * key weights stay in float32: |dw| <= 2 DS sum g + 1e-6 w, summed over the rows,
 with g = dp/ds up to the threshold's own error: p (softmax1), 1[z > tau - 2 DS]
@@ -25,7 +25,8 @@ from hf_attention_normalizers_b200 import serving
 pytestmark = pytest.mark.gpu
 
 NORMS = ("softmax1", "sparsemax", "entmax15")
-UNIT = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -12, torch.bfloat16: 2.0 ** -9}
+# half the spacing of 1 + eps: significands of 24, 11 and 8 bits
+UNIT = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.float16, torch.bfloat16)}
 
 
 class Batch:
