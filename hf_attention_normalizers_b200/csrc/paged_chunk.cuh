@@ -88,4 +88,27 @@ __device__ __forceinline__ void load_key_tile_tma(uint8_t* stage, const CUtensor
   }
 }
 
+// ------------------------------------------------------------------ host
+inline int sm_count() {
+  static int n[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n[dev];
+}
+
+// (dim, head, token) map of packed rows: a box is one tile, rows token-major.
+inline bool make_row_map(CUtensorMap* m, const AttnParams& p, bool bf16, const ChunkPlan& c) {
+  return tc::make_map_box(m, p.q, bf16, {(cuuint64_t)p.d, (cuuint64_t)p.hq, (cuuint64_t)p.rows_total, 1},
+                      {p.q_sh, p.q_st, p.q_st * p.rows_total}, {64, (cuuint32_t)c.group, (cuuint32_t)c.tpb, 1});
+}
+inline bool make_page_map(CUtensorMap* m, const void* cache, int64_t st, int64_t sh, const AttnParams& p, bool bf16,
+                   const ChunkPlan& c) {
+  return tc::make_map(m, cache, bf16, p.d, p.num_cache_tokens, p.hkv, 1, st, sh, p.num_cache_tokens * st, c.box_rows);
+}
+
+// Thresholds of the sparse normalizers into p.stats, and the output of every
+// unit whose flag it leaves 0 (flags [pairs][hkv]).
+cudaError_t chunk_sparse_scan(int dtype, const AttnParams& p, const ChunkPlan& c, int* flags, cudaStream_t s);
+
 }  // namespace hfan

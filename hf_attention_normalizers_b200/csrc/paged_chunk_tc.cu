@@ -72,6 +72,7 @@ struct ChunkWs {
   float* o;    // [splits][total_q * hq][D]
   float2* ml;  // [splits][total_q * hq]
   int* parts;  // [total_q * hq] parts that the row has (1: already final)
+  int* flags;  // sparse: [pairs][hkv], 0 where the scan has written the output
 };
 
 __device__ __forceinline__ void fail(const AttnParams& p, ChunkCtl* ctl) {
@@ -99,6 +100,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (!find_group(p, 2 * c.tpb, blockIdx.x, &b, &pair)) return;
   const Geometry g = geometry(p, b);
   const int kvh = blockIdx.y, split = blockIdx.z;
+  if (NORM != HFAN_SOFTMAX1 && ws.flags[blockIdx.x * p.hkv + kvh] == 0) return;
   const int tok0 = pair * 2 * c.tpb, ntok = min(2 * c.tpb, g.q_len - tok0);
   const int nact = ntok > c.tpb ? 2 : 1;  // tiles with rows
   const int k_hi = p.causal ? min(g.k_len, tok0 + ntok + g.shift) : g.k_len;
@@ -624,14 +626,6 @@ int pow2_divisor(int n, int most) {
   return r;
 }
 
-int sm_count() {
-  static int n[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n[dev];
-}
-
 ChunkPlan plan_of(const AttnParams& p) {
   ChunkPlan c;
   c.group = p.hq / p.hkv;
@@ -643,6 +637,12 @@ ChunkPlan plan_of(const AttnParams& p) {
   const int64_t pairs = p.rows_total / (2 * c.tpb) + (p.batch < p.rows_total ? p.batch : p.rows_total);
   c.pairs = (int)(pairs < 1 ? 1 : pairs);
   const int ktiles = (p.len_k + kTileKeys - 1) / kTileKeys;
+  // Sparse: this kernel serves what the scan flagged, which nobody knows yet.
+  if (p.norm != HFAN_SOFTMAX1) {
+    c.splits = 1;
+    c.span = ktiles > 0 ? ktiles : 1;
+    return c;
+  }
   // One wave of CTAs over the SMs; a part shorter than four key tiles would
   // pay more for its prologue and its partial result than it saves.
   const int64_t units = (int64_t)c.pairs * p.hkv;
@@ -657,27 +657,18 @@ ChunkPlan plan_of(const AttnParams& p) {
 }
 
 struct WsLayout {
-  int64_t o, ml, parts, total;
+  int64_t o, ml, parts, flags, total;
 };
 WsLayout ws_layout(const AttnParams& p, const ChunkPlan& c) {
   auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
   const int64_t rows = (int64_t)p.rows_total * p.hq;
-  WsLayout w{0, 0, 0, 0};
+  WsLayout w{0, 0, 0, 0, 0};
+  if (p.norm != HFAN_SOFTMAX1) w.total = up((int64_t)c.pairs * p.hkv * 4);
   if (c.splits < 2) return w;
   w.ml = up(rows * c.splits * p.d * 4);
   w.parts = w.ml + up(rows * c.splits * 8);
   w.total = w.parts + up(rows * 4);
   return w;
-}
-
-// (dim, head, token) map of packed rows: a box is one tile, rows token-major.
-bool make_row_map(CUtensorMap* m, const AttnParams& p, bool bf16, const ChunkPlan& c) {
-  return make_map_box(m, p.q, bf16, {(cuuint64_t)p.d, (cuuint64_t)p.hq, (cuuint64_t)p.rows_total, 1},
-                      {p.q_sh, p.q_st, p.q_st * p.rows_total}, {64, (cuuint32_t)c.group, (cuuint32_t)c.tpb, 1});
-}
-bool make_page_map(CUtensorMap* m, const void* cache, int64_t st, int64_t sh, const AttnParams& p, bool bf16,
-                   const ChunkPlan& c) {
-  return make_map(m, cache, bf16, p.d, p.num_cache_tokens, p.hkv, 1, st, sh, p.num_cache_tokens * st, c.box_rows);
 }
 
 template <int HD, bool BF16, int NORM>
@@ -687,12 +678,17 @@ cudaError_t fwd_t(const AttnParams& p, const ChunkPlan& c, void* workspace, cuda
       !make_page_map(&tv, p.v, p.v_st, p.v_sh, p, BF16, c))
     return cudaErrorInvalidValue;
   const WsLayout w = ws_layout(p, c);
-  ChunkWs ws{nullptr, nullptr, nullptr};
+  ChunkWs ws{nullptr, nullptr, nullptr, nullptr};
   if (c.splits > 1) {
     uint8_t* base = static_cast<uint8_t*>(workspace);
     ws.o = reinterpret_cast<float*>(base + w.o);
     ws.ml = reinterpret_cast<float2*>(base + w.ml);
     ws.parts = reinterpret_cast<int*>(base + w.parts);
+  }
+  if (NORM != HFAN_SOFTMAX1) {
+    ws.flags = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + w.flags);
+    const cudaError_t e = chunk_sparse_scan(BF16 ? HFAN_BFLOAT16 : HFAN_FLOAT16, p, c, ws.flags, s);
+    if (e != cudaSuccess) return e;
   }
   auto kernel = chunk_fwd_kernel<HD, BF16, NORM>;
   constexpr int smem = ChunkLayout<HD>::TOTAL;
@@ -748,7 +744,7 @@ bool keys_supported(int dtype, const AttnParams& p) {
 }  // namespace
 
 bool chunk_tc_supported(int dtype, const AttnParams& p) {
-  return p.norm == HFAN_SOFTMAX1 && keys_supported(dtype, p) && aligned16(p.v) && aligned16(p.o) && stride_ok(p.v_st) &&
+  return keys_supported(dtype, p) && aligned16(p.v) && aligned16(p.o) && stride_ok(p.v_st) &&
          stride_ok(p.v_sh) && p.o_st % 8 == 0 && p.o_sh % 8 == 0;
 }
 
