@@ -7,6 +7,8 @@
 // and every byte of K and V serves the whole group.
 #pragma once
 
+#include <atomic>
+
 #include "params.cuh"
 #include "tc_common.cuh"
 
@@ -95,6 +97,21 @@ inline int sm_count() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
   if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
   return n[dev];
+}
+
+// Lets `kernel` use `smem` bytes of dynamic shared memory: once per kernel and
+// device (the attribute call costs a launch about as much as its arguments).
+template <auto Kernel>
+cudaError_t allow_smem(int smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // (dim, head, token) map of packed rows: a box is one tile, rows token-major.

@@ -535,7 +535,7 @@ cudaError_t run(const AttnParams& p, const ChunkPlan& c, int ranks, int* flags, 
     return cudaErrorInvalidValue;
   auto kernel = chunk_sparse_kernel<HD, BF16, NORM>;
   constexpr int smem = SparseLayout<HD>::TOTAL;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<chunk_sparse_kernel<HD, BF16, NORM>>(smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c.pairs * ranks, p.hkv, 1);

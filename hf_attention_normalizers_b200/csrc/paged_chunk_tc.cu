@@ -692,7 +692,7 @@ cudaError_t fwd_t(const AttnParams& p, const ChunkPlan& c, void* workspace, cuda
   }
   auto kernel = chunk_fwd_kernel<HD, BF16, NORM>;
   constexpr int smem = ChunkLayout<HD>::TOTAL;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<chunk_fwd_kernel<HD, BF16, NORM>>(smem);
   if (e != cudaSuccess) return e;
   kernel<<<dim3(c.pairs, p.hkv, c.splits), kChunkThreads, smem, s>>>(tq, tk, tv, p, c, ws);
   if (c.splits > 1) {
@@ -710,7 +710,7 @@ cudaError_t weights_t(const AttnParams& p, const ChunkPlan& c, float* kw, int64_
     return cudaErrorInvalidValue;
   auto kernel = chunk_weights_kernel<HD, BF16, NORM>;
   constexpr int smem = WeightLayout<HD>::TOTAL;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<chunk_weights_kernel<HD, BF16, NORM>>(smem);
   if (e != cudaSuccess) return e;
   kernel<<<dim3((p.len_k + kTileKeys - 1) / kTileKeys, p.hkv, p.batch), kWeightThreads, smem, s>>>(tq, tk, p, c, kw, ldw);
   return cudaGetLastError();

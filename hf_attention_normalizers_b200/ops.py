@@ -5,7 +5,7 @@ Ops (namespace ``hfan``):
   attn_fwd / attn_bwd       dense [B, H, S, D] attention
   varlen_fwd / varlen_bwd   packed [T, H, D] attention with cu_seqlens
   paged_fwd / paged_bwd     paged KV cache + block_table
-  paged_append, paged_chunk_fwd, paged_key_weights, paged_evict
+  paged_append, paged_chunk_fwd, paged_evict
                             paged serving (inference only; the caches are
                             written in place)
   rownorm_fwd / rownorm_bwd row normalizers on a materialised matrix
@@ -488,91 +488,103 @@ torch.library.register_autograd("hfan::paged_fwd", _paged_backward, setup_contex
 # layer, and the op dispatch costs as much host time as the whole launch, so
 # eager callers (serving.py) use the functions.
 # ---------------------------------------------------------------------------
-def _chunk_desc(dtype, normalizer, batch, heads_q, heads_kv, head_dim, total_q, max_q, page_size, max_k, cache_tokens,
-                block_table, cu, seq_lens, scale, causal) -> N.ChunkDesc:
-    # positional: field order of hfan_chunk_desc
-    return N.ChunkDesc(dtype, normalizer, batch, heads_q, heads_kv, head_dim, total_q, max_q, page_size,
-                       block_table.shape[1], max_k, cache_tokens, block_table.data_ptr(),
-                       None if cu is None else cu.data_ptr(), seq_lens.data_ptr(), scale, causal)
+_Desc, _View = N.ChunkDesc, N.HfanTensor
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _i32(t: Tensor) -> Tensor:
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _rows3(t: Tensor) -> N.HfanTensor:
+    """``_t3`` of a tensor whose innermost stride is known to be one."""
+    s = t.stride()
+    return _View(t.data_ptr(), 0, s[1], s[0])
+
+
+def _elsewhere(t: Tensor) -> bool:
+    """Whether t lives on another device than the current one (the launch then needs a device guard)."""
+    return t.get_device() != torch.cuda.current_device()
 
 
 def launch_paged_append(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: Tensor, block_table: Tensor,
                         cu_seqlens: Tensor, seq_lens: Tensor, page_size: int, max_q: int,
                         key_weights: Optional[Tensor]) -> None:
-    _require_cuda(key, value, key_cache, value_cache, block_table, cu_seqlens, seq_lens)
+    if _elsewhere(key):
+        with torch.cuda.device(key.device):
+            return launch_paged_append(key, value, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size,
+                                       max_q, key_weights)
     key, value = _inner_contig(key), _inner_contig(value)
     bt, cu, sl = _i32(block_table), _i32(cu_seqlens), _i32(seq_lens)
     total, hkv, d = key.shape
-    desc = _chunk_desc(dtype_id(key), N.SOFTMAX1, bt.shape[0], hkv, hkv, d, total, max_q, page_size,
-                       bt.shape[1] * page_size, key_cache.shape[0], bt, cu, sl, 1.0, 1)
-    with torch.cuda.device(key.device):
-        N.check(N.lib().hfan_paged_append(ctypes.byref(desc), _t3(key), _t3(value), _t3(key_cache), _t3(value_cache),
-                                          _ptr(key_weights), 0 if key_weights is None else key_weights.stride(0),
-                                          _stream(key)), "hfan_paged_append")
+    batch, cols = bt.shape
+    desc = _Desc(dtype_id(key), N.SOFTMAX1, batch, hkv, hkv, d, total, max_q, page_size, cols, cols * page_size,
+                 key_cache.shape[0], bt.data_ptr(), cu.data_ptr(), sl.data_ptr(), 1.0, 1)
+    kw, ld = (None, 0) if key_weights is None else (key_weights.data_ptr(), key_weights.stride(0))
+    rc = N.lib().hfan_paged_append(ctypes.byref(desc), _rows3(key), _rows3(value), _rows3(key_cache),
+                                   _rows3(value_cache), kw, ld, _raw_stream(key.get_device()))
+    if rc:
+        N.check(rc, "hfan_paged_append")
 
 
 def launch_paged_chunk_fwd(q: Tensor, key_cache: Tensor, value_cache: Tensor, block_table: Tensor, cu_seqlens: Tensor,
                            seq_lens: Tensor, page_size: int, max_q: int, max_k: int, normalizer: int, scale: float,
-                           causal: bool) -> tuple[Tensor, Tensor]:
-    """Returns (o [T, Hq, D], stats float32 [2, Hq, T])."""
-    _require_cuda(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens)
+                           causal: bool, key_weights: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
+    """Returns (o [T, Hq, D], stats float32 [2, Hq, T]); adds to ``key_weights`` when it is given."""
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return launch_paged_chunk_fwd(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q,
+                                          max_k, normalizer, scale, causal, key_weights)
     q = _inner_contig(q)
     bt, cu, sl = _i32(block_table), _i32(cu_seqlens), _i32(seq_lens)
     total, hq, d = q.shape
-    o = torch.empty((total, hq, d), dtype=q.dtype, device=q.device)
+    batch, cols = bt.shape
+    slots, hkv, _ = key_cache.shape
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     stats = torch.empty((2, hq, total), dtype=torch.float32, device=q.device)
-    desc = _chunk_desc(dtype_id(q), normalizer, bt.shape[0], hq, key_cache.shape[1], d, total, max_q, page_size, max_k,
-                       key_cache.shape[0], bt, cu, sl, scale, causal)
-    lib = N.lib()
-    with torch.cuda.device(q.device):
-        nbytes = lib.hfan_paged_chunk_workspace_bytes(ctypes.byref(desc))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-        N.check(lib.hfan_paged_chunk_fwd(ctypes.byref(desc), _t3(q), _t3(key_cache), _t3(value_cache), _t3(o),
-                                         _ptr(stats), _ptr(ws), max(nbytes, 0), _stream(q)), "hfan_paged_chunk_fwd")
+    desc = _Desc(dtype_id(q), normalizer, batch, hq, hkv, d, total, max_q, page_size, cols, max_k, slots, bt.data_ptr(),
+                 cu.data_ptr(), sl.data_ptr(), scale, causal)
+    lib, ref, qv, kv, stream = N.lib(), ctypes.byref(desc), _rows3(q), _rows3(key_cache), _raw_stream(q.get_device())
+    nbytes = lib.hfan_paged_chunk_workspace_bytes(ref)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    sp = stats.data_ptr()
+    rc = lib.hfan_paged_chunk_fwd(ref, qv, kv, _rows3(value_cache), _rows3(o), sp, None if ws is None else ws.data_ptr(),
+                                  nbytes if nbytes > 0 else 0, stream)
+    if rc:
+        N.check(rc, "hfan_paged_chunk_fwd")
+    if key_weights is not None:
+        rc = lib.hfan_paged_key_weights(ref, qv, kv, sp, key_weights.data_ptr(), key_weights.stride(0), stream)
+        if rc:
+            N.check(rc, "hfan_paged_key_weights")
     return o, stats
-
-
-def launch_paged_key_weights(q: Tensor, key_cache: Tensor, stats: Tensor, block_table: Tensor, cu_seqlens: Tensor,
-                             seq_lens: Tensor, page_size: int, max_q: int, max_k: int, normalizer: int, scale: float,
-                             causal: bool, key_weights: Tensor) -> None:
-    _require_cuda(q, key_cache, stats, block_table, cu_seqlens, seq_lens, key_weights)
-    q = _inner_contig(q)
-    bt, cu, sl = _i32(block_table), _i32(cu_seqlens), _i32(seq_lens)
-    total, hq, d = q.shape
-    desc = _chunk_desc(dtype_id(q), normalizer, bt.shape[0], hq, key_cache.shape[1], d, total, max_q, page_size, max_k,
-                       key_cache.shape[0], bt, cu, sl, scale, causal)
-    with torch.cuda.device(q.device):
-        N.check(N.lib().hfan_paged_key_weights(ctypes.byref(desc), _t3(q), _t3(key_cache), _ptr(stats),
-                                               _ptr(key_weights), key_weights.stride(0), _stream(q)),
-                "hfan_paged_key_weights")
 
 
 def launch_paged_evict(key_cache: Tensor, value_cache: Tensor, key_weights: Tensor, block_table: Tensor,
                        seq_lens: Tensor, page_size: int, max_k: int, budget: int, recent: int) -> tuple[Tensor, Tensor]:
     """Returns (lengths int32 [B], kept int32 [B, Hkv, budget])."""
-    _require_cuda(key_cache, value_cache, key_weights, block_table, seq_lens)
+    if _elsewhere(key_cache):
+        with torch.cuda.device(key_cache.device):
+            return launch_paged_evict(key_cache, value_cache, key_weights, block_table, seq_lens, page_size, max_k, budget,
+                                      recent)
     bt, sl = _i32(block_table), _i32(seq_lens)
-    tokens, hkv, d = key_cache.shape
-    kept = torch.empty((bt.shape[0], hkv, budget), dtype=torch.int32, device=key_cache.device)
-    lens = torch.empty((bt.shape[0],), dtype=torch.int32, device=key_cache.device)
-    desc = _chunk_desc(dtype_id(key_cache), N.SOFTMAX1, bt.shape[0], hkv, hkv, d, 0, 0, page_size, max_k, tokens, bt,
-                       None, sl, 1.0, 1)
-    with torch.cuda.device(key_cache.device):
-        N.check(N.lib().hfan_paged_evict(ctypes.byref(desc), _t3(key_cache), _t3(value_cache), _ptr(key_weights),
-                                         key_weights.stride(0), budget, recent, _ptr(kept), _ptr(lens),
-                                         _stream(key_cache)), "hfan_paged_evict")
+    slots, hkv, d = key_cache.shape
+    batch, cols = bt.shape
+    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=key_cache.device)
+    lens = torch.empty((batch,), dtype=torch.int32, device=key_cache.device)
+    desc = _Desc(dtype_id(key_cache), N.SOFTMAX1, batch, hkv, hkv, d, 0, 0, page_size, cols, max_k, slots, bt.data_ptr(),
+                 None, sl.data_ptr(), 1.0, 1)
+    rc = N.lib().hfan_paged_evict(ctypes.byref(desc), _rows3(key_cache), _rows3(value_cache), key_weights.data_ptr(),
+                                  key_weights.stride(0), budget, recent, kept.data_ptr(), lens.data_ptr(),
+                                  _raw_stream(key_cache.get_device()))
+    if rc:
+        N.check(rc, "hfan_paged_evict")
     return lens, kept
 
 
 paged_append = torch.library.custom_op(
     "hfan::paged_append", launch_paged_append, mutates_args=("key_cache", "value_cache", "key_weights"))
-paged_chunk_fwd = torch.library.custom_op("hfan::paged_chunk_fwd", launch_paged_chunk_fwd, mutates_args=())
-paged_key_weights = torch.library.custom_op(
-    "hfan::paged_key_weights", launch_paged_key_weights, mutates_args=("key_weights",))
+paged_chunk_fwd = torch.library.custom_op(
+    "hfan::paged_chunk_fwd", launch_paged_chunk_fwd, mutates_args=("key_weights",))
 paged_evict = torch.library.custom_op(
     "hfan::paged_evict", launch_paged_evict, mutates_args=("key_cache", "value_cache", "key_weights"))
 
@@ -583,14 +595,9 @@ def _(key, value, key_cache, value_cache, block_table, cu_seqlens, seq_lens, pag
 
 
 @paged_chunk_fwd.register_fake
-def _(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q, max_k, normalizer, scale, causal):
+def _(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q, max_k, normalizer, scale, causal,
+      key_weights=None):
     return (q.new_empty(q.shape), q.new_empty((2, q.shape[1], q.shape[0]), dtype=torch.float32))
-
-
-@paged_key_weights.register_fake
-def _(q, key_cache, stats, block_table, cu_seqlens, seq_lens, page_size, max_q, max_k, normalizer, scale, causal,
-      key_weights):
-    return None
 
 
 @paged_evict.register_fake

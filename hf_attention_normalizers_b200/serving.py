@@ -42,49 +42,53 @@ from .paged import _normalizer_name
 __all__ = ["paged_append", "paged_chunk_attention", "paged_evict", "device_status"]
 
 
+_INTS = (torch.int32, torch.int64)
+
+
 def _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights, name) -> None:
-    if key_cache.ndim != 3 or key_cache.shape != value_cache.shape:
+    shape, tables, lens = key_cache.shape, block_table.shape, sequence_lengths.shape
+    if len(shape) != 3 or shape != value_cache.shape:
         raise ValueError("key_cache/value_cache must have matching [pages, heads, dim] shapes.")
-    if key_cache.dtype != value_cache.dtype:
+    if key_cache.dtype is not value_cache.dtype:
         raise ValueError("key_cache and value_cache must have one dtype.")
     if key_cache.stride(2) != 1 or value_cache.stride(2) != 1:
         raise ValueError("key_cache/value_cache must have a unit innermost stride.")
     if not key_cache.is_cuda or not value_cache.is_cuda:
         raise ValueError(f"{name} requires CUDA tensors.")
-    if block_table.ndim != 2:
+    if len(tables) != 2:
         raise ValueError("block_table must have shape [batch, max_blocks].")
-    if sequence_lengths.ndim != 1 or sequence_lengths.shape[0] != block_table.shape[0]:
+    if len(lens) != 1 or lens[0] != tables[0]:
         raise ValueError("sequence_lengths must have shape [batch].")
-    if block_table.shape[0] < 1:
+    if tables[0] < 1:
         raise ValueError("The batch must hold at least one sequence.")
-    for t, what in ((block_table, "block_table"), (sequence_lengths, "sequence_lengths")):
-        if t.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{what} must use int32 or int64.")
+    if block_table.dtype not in _INTS or sequence_lengths.dtype not in _INTS:
+        raise ValueError("block_table and sequence_lengths must use int32 or int64.")
     if block_size <= 0:
         raise ValueError("block_size must be positive.")
     if key_weights is not None:
-        if key_weights.dtype != torch.float32 or key_weights.shape != (key_cache.shape[1], key_cache.shape[0]):
+        if key_weights.dtype is not torch.float32 or key_weights.shape != (shape[1], shape[0]):
             raise ValueError("key_weights must be float32 [kv_heads, num_blocks * block_size].")
-        if key_weights.stride(1) != 1 or key_weights.stride(0) < key_weights.shape[1]:
+        if key_weights.stride(1) != 1 or key_weights.stride(0) < shape[0]:
             raise ValueError("key_weights must have contiguous rows.")
 
 
 def _check_rows(rows, key_cache, cu_seqlens, block_table, name) -> None:
-    if cu_seqlens.ndim != 1 or cu_seqlens.numel() != block_table.shape[0] + 1:
+    if cu_seqlens.shape != (block_table.shape[0] + 1,):
         raise ValueError(f"{name} must have shape [batch + 1].")
-    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+    if cu_seqlens.dtype not in _INTS:
         raise ValueError(f"{name} must use int32 or int64.")
-    if rows.dtype != key_cache.dtype:
+    if rows.dtype is not key_cache.dtype:
         raise ValueError("New tokens and cache must have one dtype.")
     if rows.shape[-1] != key_cache.shape[-1]:
         raise ValueError("New tokens and cache head dimensions must match.")
 
 
-def _check_devices(first, *others) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
+def _check_placement(*tensors) -> None:
+    where = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != where:
             raise ValueError("All tensors must be on one device.")
-    if torch.is_grad_enabled() and (first.requires_grad or any(t is not None and t.requires_grad for t in others)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError("Paged serving is inference only: call it under torch.no_grad() or detach its inputs.")
 
 
@@ -112,7 +116,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     if key.shape[1] != key_cache.shape[1]:
         raise ValueError("New keys and cache must have the same KV heads.")
     _check_rows(key, key_cache, cu_seqlens, block_table, "cu_seqlens")
-    _check_devices(key_cache, value_cache, key, value, block_table, cu_seqlens, sequence_lengths, key_weights)
+    _check_placement(key_cache, value_cache, key, value, block_table, cu_seqlens, sequence_lengths, key_weights)
     call = ops.paged_append if torch.compiler.is_compiling() else ops.launch_paged_append
     call(key, value, key_cache, value_cache, block_table, cu_seqlens, sequence_lengths, int(block_size), key.shape[0],
          key_weights)
@@ -139,20 +143,16 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     if query.shape[1] % key_cache.shape[1] != 0:
         raise ValueError("query heads must be divisible by KV heads.")
     _check_rows(query, key_cache, cu_seqlens_q, block_table, "cu_seqlens_q")
-    _check_devices(key_cache, value_cache, query, block_table, cu_seqlens_q, sequence_lengths, key_weights)
-    norm = N.NORMALIZER_IDS[_normalizer_name(normalizer)]
+    _check_placement(key_cache, value_cache, query, block_table, cu_seqlens_q, sequence_lengths, key_weights)
+    norm = N.NORMALIZER_IDS.get(normalizer) if isinstance(normalizer, str) else None
+    if norm is None:
+        norm = N.NORMALIZER_IDS[_normalizer_name(normalizer)]
     max_q = _bound(max_seqlen_q, query.shape[0], "max_seqlen_q")
     max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
     actual_scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
-    compiling = torch.compiler.is_compiling()
-    o, stats = (ops.paged_chunk_fwd if compiling else ops.launch_paged_chunk_fwd)(
-        query, key_cache, value_cache, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k, norm,
-        actual_scale, bool(is_causal))
-    if key_weights is not None:
-        (ops.paged_key_weights if compiling else ops.launch_paged_key_weights)(
-            query, key_cache, stats, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k, norm,
-            actual_scale, bool(is_causal), key_weights)
-    return o
+    call = ops.paged_chunk_fwd if torch.compiler.is_compiling() else ops.launch_paged_chunk_fwd
+    return call(query, key_cache, value_cache, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k,
+                norm, actual_scale, bool(is_causal), key_weights)[0]
 
 
 def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, key_weights: torch.Tensor,
@@ -176,7 +176,7 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, key_weights:
         raise ValueError("budget must be positive.")
     if recent < 0:
         raise ValueError("recent must not be negative.")
-    _check_devices(key_cache, value_cache, block_table, sequence_lengths, key_weights)
+    _check_placement(key_cache, value_cache, block_table, sequence_lengths, key_weights)
     max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
     call = ops.paged_evict if torch.compiler.is_compiling() else ops.launch_paged_evict
     return call(key_cache, value_cache, key_weights, block_table, sequence_lengths, int(block_size), max_k, int(budget),
