@@ -50,6 +50,7 @@ struct SparseLayout {
   static constexpr uint32_t Z = K + STAGES * TILE;        // float [CAP][256]
   static constexpr uint32_t ID = Z + CAP * 256 * 4;       // uint16 [CAP][256]
   static constexpr uint32_t XCH = ID + CAP * 256 * 2;     // float4 [2][256]
+  static_assert(CAP * 256 * 4 <= (2 + STAGES) * NH * kHalf, "the rows of the support go over the Q and K tiles");
   static constexpr uint32_t CNT = XCH + 2 * 256 * 16;     // float [256] entries left above tau
   static constexpr uint32_t BARS = CNT + 256 * 4;
   static constexpr uint32_t TOTAL = BARS + 512 + 1024;
@@ -77,14 +78,35 @@ struct Scan {
   float gate;  // the same in raw scores, or slightly below
 };
 
-// Raises thr to the threshold of the buffered entries alone (their sum never
-// exceeds the row's) and drops the dead ones.
+// Raises thr towards the threshold of the buffered entries alone (their sum
+// never exceeds the row's, and the steps never overshoot) and drops the dead.
+// z, id: shared-space addresses of the row's columns, entries kZStep and
+// kIdStep bytes apart.
+constexpr uint32_t kZStep = 256 * 4, kIdStep = 256 * 2;
+
+__device__ __forceinline__ int drop_dead(uint32_t z, uint32_t id, int n, float t) {
+  int live = 0;
+#pragma unroll 4
+  for (int e = 0; e < n; ++e) {
+    const float x = lds_f32(z + e * kZStep);
+    const uint32_t k = lds_u16(id + e * kIdStep);
+    const bool in = x > t;
+    sts_f32_if(in, z + live * kZStep, x);
+    sts_u16_if(in, id + live * kIdStep, k);
+    live += in ? 1 : 0;
+  }
+  return live;
+}
+
 template <int NORM>
-__device__ __noinline__ Scan compact(float* z, uint16_t* id, Scan s, int cap, float izs) {
+__device__ __noinline__ Scan compact(uint32_t z, uint32_t id, Scan s, int cap, float izs) {
+  if (s.over) return s;
   float t = s.thr, tau = s.thr;
-  for (int it = 0; it < 8; ++it) {
+#pragma unroll 1
+  for (int it = 0; it < 3; ++it) {
     TauStats st{0.f, 0.f, 0.f, kPosInf};
-    for (int e = 0; e < s.n; ++e) tau_accumulate(st, z[e * 256], t);
+#pragma unroll 4
+    for (int e = 0; e < s.n; ++e) tau_accumulate(st, lds_f32(z + e * kZStep), t);
     if (st.cnt == 0.f) break;
     if (tau_step(NORM, st, &t, &tau)) {
       t = tau;
@@ -95,16 +117,8 @@ __device__ __noinline__ Scan compact(float* z, uint16_t* id, Scan s, int cap, fl
     s.thr = t;
     s.gate = raw_gate(t, izs);
   }
-  int live = 0;
-  for (int e = 0; e < s.n; ++e) {
-    const float x = z[e * 256];
-    if (x > s.thr) {
-      id[live * 256] = id[e * 256];
-      z[live++ * 256] = x;
-    }
-  }
-  s.n = live;
-  if (live > cap - 12) s.over = true;  // no room for a chunk of eight
+  s.n = drop_dead(z, id, s.n, s.thr);
+  if (s.n > cap - 12) s.over = true;  // no room for a chunk of eight
   return s;
 }
 
@@ -239,8 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.causal && row_ok) vis = min(vis, i + g.shift + 1);
     const bool warp_on = __any_sync(0xffffffffu, vis > kt0 * kTileKeys);
     const float zs = NORM == HFAN_SPARSEMAX ? p.scale : 0.5f * p.scale, izs = 1.f / zs;
-    float* zb = reinterpret_cast<float*>(smem + L::Z) + slot;
-    uint16_t* ib = reinterpret_cast<uint16_t*>(smem + L::ID) + slot;
+    const uint32_t zb = smem_u32(smem + L::Z) + slot * 4, ib = smem_u32(smem + L::ID) + slot * 2;
     float4* xch = reinterpret_cast<float4*>(smem + L::XCH);
     bool ok = true;
     int it = 0, rounds = 0;
@@ -255,20 +268,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       warp_arrive(&bars->s_empty[q][it & 1]);
       ++it;
     };
-    // 32 scores of tile t from column cc * 32, masked ones -inf
-    auto load32 = [&](int t, int cc, float (&s)[32]) {
-      uint32_t x[32];
-      tmem_ld32(s_col + (it & 1) * 128 + cc * 32, x);
-      tmem_wait_ld();
+    // scores of columns [32 cc, 32 cc + 32) of tile t, masked ones -inf
+    auto mask32 = [&](int t, int cc, uint32_t (&x)[32]) {
       const int lim = vis - (kt0 + t) * kTileKeys - cc * 32;
-      if (__all_sync(0xffffffffu, lim >= 32)) {
+      if (!__all_sync(0xffffffffu, lim >= 32)) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = __uint_as_float(x[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = j < lim ? __uint_as_float(x[j]) : kNegInf;
+        for (int j = 0; j < 32; ++j) x[j] = j < lim ? x[j] : 0xff800000u;
       }
     };
+    auto s_at = [&](int cc) { return s_col + (it & 1) * 128 + cc * 32; };
     // Publishes v and visits every rank's value of the same row in rank order.
     // Two buffers suffice: a warp writes one again only after its counterparts
     // arrived for the other, which they do when they have read this one.
@@ -289,69 +297,88 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- scan
     Scan sc{0, false, kNegInf, kNegInf};
-    float zmax = kNegInf;
-    float tk[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+    float smax = kNegInf;
+    float tk[4] = {kNegInf, kNegInf, kNegInf, kNegInf};  // the largest 8-key maxima
+    auto raise = [&]() {
+      if (tk[0] > kNegInf) {
+        const float zk[4] = {tk[0] * zs, tk[1] * zs, tk[2] * zs, tk[3] * zs};
+        const float lb = top_bound<NORM, 4>(zk);
+        if (lb > sc.thr) {
+          sc.thr = lb;
+          sc.gate = raw_gate(lb, izs);
+        }
+      }
+    };
     for (int t = 0; t < nt; ++t) {
       if (!(ok = wait_s())) break;
       if (warp_on) {
-        float cm[16];
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          float s[32];
-          load32(t, cc, s);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) cm[cc * 4 + e] = max_n<8>(s + e * 8);
-        }
-        const float tm = max_n<16>(cm);
-        zmax = fmaxf(zmax, tm * zs);
-        // a tile without a score above the bound changes nothing
-        if (__any_sync(0xffffffffu, tm > sc.gate)) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float four[4] = {cm[4 * e], cm[4 * e + 1], cm[4 * e + 2], cm[4 * e + 3]};
-            top4_merge(tk, four);
-          }
-          if (tk[0] > kNegInf) {
-            const float zk[4] = {tk[0] * zs, tk[1] * zs, tk[2] * zs, tk[3] * zs};
-            const float lb = top_bound<NORM, 4>(zk);
-            if (lb > sc.thr) {
-              sc.thr = lb;
-              sc.gate = raw_gate(lb, izs);
-            }
-          }
-          uint32_t mine = 0u;  // chunks of eight with a candidate
-          if (!sc.over) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mine |= cm[e] > sc.gate ? 1u << e : 0u;
-          }
-          const int lim = vis - (kt0 + t) * kTileKeys;
-          for (uint32_t todo = __reduce_or_sync(0xffffffffu, mine); todo != 0u; todo &= todo - 1u) {
-            const int e = __ffs(todo) - 1;
-            uint32_t x[8];
-            tmem_ld8(s_col + (it & 1) * 128 + e * 8, x);
+        if (t == 0) {
+          // the first tile's maxima give a bound before anything is buffered
+#pragma unroll 1
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t x[32];
+            tmem_ld32(s_at(cc), x);
             tmem_wait_ld();
-            if ((mine >> e) & 1u) {
-              if (sc.n > CAP - 8 && !sc.over) sc = compact<NORM>(zb, ib, sc, CAP, izs);
-              if (!sc.over) {
+            mask32(t, cc, x);
+            const float* s = reinterpret_cast<const float*>(x);
+            const float cm[4] = {max_n<8>(s), max_n<8>(s + 8), max_n<8>(s + 16), max_n<8>(s + 24)};
+            top4_merge(tk, cm);
+          }
+          raise();
+          tk[0] = tk[1] = tk[2] = tk[3] = kNegInf;  // (merged again below)
+        }
+        bool heavy = false;
+#pragma unroll 1  // (unrolled, the code of a tile outgrows the instruction caches)
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t x[32];
+          tmem_ld32(s_at(cc), x);
+          tmem_wait_ld();
+          mask32(t, cc, x);
+          const float* s = reinterpret_cast<const float*>(x);
+          float hm[8], cm[4];  // maxima of four and of eight keys
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  // written at slot n, which only advances past a candidate
-                  const float s = __uint_as_float(x[j]);
-                  const bool in = s > sc.gate && e * 8 + j < lim;
-                  if (in) {
-                    zb[sc.n * 256] = s * zs;
-                    ib[sc.n * 256] = (uint16_t)(t * kTileKeys + e * 8 + j);
-                  }
-                  sc.n += in ? 1 : 0;
+          for (int e = 0; e < 8; ++e) hm[e] = max_n<4>(s + 4 * e);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cm[e] = fmaxf(hm[2 * e], hm[2 * e + 1]);
+          const float gm = fmaxf(max3f(cm[0], cm[1], cm[2]), cm[3]);
+          smax = fmaxf(smax, gm);
+          // keys at or below the bound change nothing: no candidate, and no
+          // set of them has a threshold above it
+          if (__any_sync(0xffffffffu, gm > sc.gate)) {
+            heavy = true;
+            top4_merge(tk, cm);
+            const bool tight = __any_sync(0xffffffffu, sc.n > CAP - 32 && !sc.over);  // (the group may fill a buffer)
+            const uint32_t id0 = t * kTileKeys + cc * 32;
+            uint32_t za = zb + sc.n * kZStep, ia = ib + sc.n * kIdStep;
+            float gate = sc.over ? kPosInf : sc.gate;
+            // The branches are the warp's, the pushes predicated per lane:
+            // divergent branches around them took several times as long.
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              // All lanes compact when one has to: they do it in the same time,
+              // and their raised bounds keep them from having to one by one.
+              if (e % 2 == 0 && tight) {
+                sc.n = (za - zb) / kZStep;
+                if (__any_sync(0xffffffffu, sc.n > CAP - 8 && !sc.over)) {
+                  sc = compact<NORM>(zb, ib, sc, CAP, izs);
+                  za = zb + sc.n * kZStep;
+                  ia = ib + sc.n * kIdStep;
+                  gate = sc.over ? kPosInf : sc.gate;
                 }
               }
+              if (__any_sync(0xffffffffu, hm[e] > gate)) {
+#pragma unroll
+                for (int j = 4 * e; j < 4 * e + 4; ++j) push_if_above(s[j], gate, s[j] * zs, id0 + j, za, ia, kZStep, kIdStep);
+              }
             }
-            __syncwarp();
+            sc.n = (za - zb) / kZStep;
           }
         }
+        if (heavy) raise();
       }
       free_s();
     }
+    const float zmax = smax * zs;
 
     // ---- exact threshold on the union of the ranks' buffers
     float lower = kNegInf, zrow = kNegInf;
@@ -361,22 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       lower = fmaxf(lower, v.y);
       over |= v.z != 0.f;
     });
-    auto drop = [&](float t) {
-      int live = 0;
-      for (int e = 0; e < sc.n; ++e) {
-        const float x = zb[e * 256];
-        if (x > t) {
-          ib[live * 256] = ib[e * 256];
-          zb[live++ * 256] = x;
-        }
-      }
-      sc.n = live;
-    };
     const bool empty = !(zrow > kNegInf);
     float tau = kPosInf, support = 0.f;
     bool pending = !empty && over;
     if (!over) {
-      drop(lower);
+      sc.n = drop_dead(zb, ib, sc.n, lower);
     } else {
       sc.n = 0;
     }
@@ -385,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int step = 0; step < 64 && __any_sync(0xffffffffu, solving) && ok; ++step) {
       TauStats st{0.f, 0.f, 0.f, kPosInf}, all{0.f, 0.f, 0.f, kPosInf};
       if (solving)
-        for (int e = 0; e < sc.n; ++e) tau_accumulate_ref(st, zb[e * 256], lower, zrow);
+#pragma unroll 4
+        for (int e = 0; e < sc.n; ++e) tau_accumulate_ref(st, lds_f32(zb + e * kZStep), lower, zrow);
       exchange(make_float4(st.cnt, st.s1, st.s2, st.zmin), [&](float4 v) {
         all.cnt += v.x;
         all.s1 += v.y;
@@ -420,11 +437,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < nt && ok; ++t) {
         if (!(ok = wait_s())) break;
         if (__any_sync(0xffffffffu, pending)) {
+#pragma unroll 1
           for (int cc = 0; cc < 4; ++cc) {
-            float s[32];
-            load32(t, cc, s);
+            uint32_t x[32];
+            tmem_ld32(s_at(cc), x);
+            tmem_wait_ld();
+            mask32(t, cc, x);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) tau_accumulate_ref(st, s[j] * zs, lower, zrow);
+            for (int j = 0; j < 32; ++j) tau_accumulate_ref(st, __uint_as_float(x[j]) * zs, lower, zrow);
           }
         }
         free_s();
@@ -451,69 +471,77 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool dense = named_bar_or(1, row_threads, over || !ok) || per > kMaxIdTiles;
     if (threadIdx.x == 0 && rank == 0) flags[unit * p.hkv + kvh] = dense ? 1 : 0;
     if (!dense) {
+      // Every thread leaves its support in place as (p, cache row); the rows
+      // go over the Q and K tiles, which nothing reads any more.
       float* cnt = reinterpret_cast<float*>(smem + L::CNT);
-      drop(tau);
-      cnt[slot] = (float)sc.n;
+      int* rows = reinterpret_cast<int*>(smem);  // [CAP][256]
+      int live = 0;
+#pragma unroll 2
+      for (int e = 0; e < sc.n; ++e) {
+        const float d = lds_f32(zb + e * kZStep) - tau;
+        if (d > 0.f) {
+          const int64_t tok = key_token(p, g, b, kt0 * kTileKeys + (int)lds_u16(ib + e * kIdStep));
+          if (tok >= 0) {
+            sts_f32_if(true, zb + live * kZStep, NORM == HFAN_SPARSEMAX ? d : d * d);
+            rows[live++ * 256 + slot] = (int)tok;
+          }
+        }
+      }
+      cnt[slot] = (float)live;
       __syncwarp();
       if (lane < ranks) peer_arrive(&bars->lists, lane);
-      ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars->lists, 0, abort_flag));
+      if (!mbar_wait_cluster(&bars->lists, 0, abort_flag)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      // Groups of eight lanes take a row each (16 head dims of a lane at HD =
+      // 128), four rows of the warp at a time; the ranks share the rows.
+      constexpr int N = HD / 8, V = N / 8;  // values and 16-byte loads of a lane
       const float* z0 = reinterpret_cast<const float*>(smem + L::Z);
-      const uint16_t* i0 = reinterpret_cast<const uint16_t*>(smem + L::ID);
-      // The rows of this warp, dealt to the ranks.  tau of a row is in its
-      // thread's registers, so each warp serves its own 32 rows.
-      const T* vbase = static_cast<const T*>(p.v) + (int64_t)kvh * p.v_sh;
-      for (int rr = rank; rr < 32 && ok; rr += ranks) {
-        const int rs = warp * 32 + rr;
-        if (!__shfl_sync(0xffffffffu, row_ok ? 1 : 0, rr)) continue;
-        const float rt = __shfl_sync(0xffffffffu, tau, rr);
+      const T* vbase = static_cast<const T*>(p.v) + (int64_t)kvh * p.v_sh + (lane & 7) * N;
+      for (int r0 = rank * 4; r0 < 32 && ok; r0 += ranks * 4) {
+        const int rr = r0 + (lane >> 3), rs = warp * 32 + rr;
+        const bool on = __shfl_sync(0xffffffffu, row_ok ? 1 : 0, rr) != 0;
         const int ri = __shfl_sync(0xffffffffu, i, rr), rh = __shfl_sync(0xffffffffu, h, rr);
-        constexpr int N = HD / 32;
-        float acc[N];
+        uint64_t acc[N / 2];
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = 0.f;
-        for (int k = 0; k < ranks; ++k) {
+        for (int e = 0; e < N / 2; ++e) acc[e] = 0ull;
+        for (int k = 0; on && k < ranks; ++k) {
           const int n = (int)(ranks == 1 ? cnt[rs] : peer_ldf(&cnt[rs], k));
-          for (int e0 = 0; e0 < n; e0 += 32) {
-            // lane e: probability and cache row of entry e0 + e
-            float pe = 0.f;
-            int64_t off = 0;
-            if (e0 + lane < n) {
-              const int at = (e0 + lane) * 256 + rs;
-              const float d = (ranks == 1 ? z0[at] : peer_ldf(&z0[at], k)) - rt;
-              const int key = k * per * kTileKeys + (int)(ranks == 1 ? i0[at] : peer_ldu16(&i0[at], k));
-              const int64_t tok = key_token(p, g, b, key);
-              pe = tok >= 0 ? (NORM == HFAN_SPARSEMAX ? d : d * d) : 0.f;
-              off = tok >= 0 ? tok * p.v_st : 0;
+#pragma unroll 4
+          for (int e = 0; e < n; ++e) {
+            float pr;
+            int row;
+            if (ranks == 1) {
+              pr = z0[e * 256 + rs];
+              row = rows[e * 256 + rs];
+            } else {
+              pr = peer_ldf(&z0[e * 256 + rs], k);
+              row = __float_as_int(peer_ldf(reinterpret_cast<const float*>(&rows[e * 256 + rs]), k));
             }
-            const int m = min(32, n - e0);
-#pragma unroll 8
-            for (int e = 0; e < m; ++e) {
-              const float pr = __shfl_sync(0xffffffffu, pe, e);
-              const int64_t o = __shfl_sync(0xffffffffu, off, e);
-              const T* v = vbase + o + lane * N;
-              if constexpr (N == 4) {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(v));
-                const T* xe = reinterpret_cast<const T*>(&x);
+            const uint4* v = reinterpret_cast<const uint4*>(vbase + (int64_t)row * p.v_st);
+            const uint64_t p2 = f2_pack(pr, pr);
+            uint4 x[V];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) acc[y] = fmaf(pr, to_f32<T>(xe[y]), acc[y]);
-              } else {
-                const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(v));
-                const T* xe = reinterpret_cast<const T*>(&x);
-                acc[0] = fmaf(pr, to_f32<T>(xe[0]), acc[0]);
-                acc[1] = fmaf(pr, to_f32<T>(xe[1]), acc[1]);
-              }
+            for (int y = 0; y < V; ++y) x[y] = __ldg(v + y);
+#pragma unroll
+            for (int y = 0; y < V; ++y) {
+              acc[4 * y + 0] = ffma2(p2, unpack2<BF16>(x[y].x), acc[4 * y + 0]);
+              acc[4 * y + 1] = ffma2(p2, unpack2<BF16>(x[y].y), acc[4 * y + 1]);
+              acc[4 * y + 2] = ffma2(p2, unpack2<BF16>(x[y].z), acc[4 * y + 2]);
+              acc[4 * y + 3] = ffma2(p2, unpack2<BF16>(x[y].w), acc[4 * y + 3]);
             }
           }
         }
-        T* dst = static_cast<T*>(p.o) + (int64_t)(g.q_start + ri) * p.o_st + (int64_t)rh * p.o_sh + lane * N;
-        if constexpr (N == 4) {
-          uint2 y;
-          y.x = pack2<BF16>(acc[0], acc[1]);
-          y.y = pack2<BF16>(acc[2], acc[3]);
-          *reinterpret_cast<uint2*>(dst) = y;
-        } else {
-          *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0], acc[1]);
+        if (on) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + (int64_t)(g.q_start + ri) * p.o_st +
+                                                (int64_t)rh * p.o_sh + (lane & 7) * N);
+#pragma unroll
+          for (int y = 0; y < V; ++y)
+            dst[y] = make_uint4(pack2<BF16>(f2_lo(acc[4 * y]), f2_hi(acc[4 * y])),
+                                pack2<BF16>(f2_lo(acc[4 * y + 1]), f2_hi(acc[4 * y + 1])),
+                                pack2<BF16>(f2_lo(acc[4 * y + 2]), f2_hi(acc[4 * y + 2])),
+                                pack2<BF16>(f2_lo(acc[4 * y + 3]), f2_hi(acc[4 * y + 3])));
         }
+        __syncwarp();
       }
       if (!ok && lane == 0) fail(p, bars);
     }
@@ -560,10 +588,11 @@ cudaError_t run_norm(const AttnParams& p, const ChunkPlan& c, int ranks, int* fl
 }  // namespace
 
 cudaError_t chunk_sparse_scan(int dtype, const AttnParams& p, const ChunkPlan& c, int* flags, cudaStream_t s) {
-  // CTAs of a cluster: as many as fill the SMs, each with four key tiles or more
+  // CTAs of a cluster: up to two waves over the SMs (the bound counts pairs
+  // that ragged sequences do not fill), each CTA with four key tiles or more
   const int64_t units = (int64_t)c.pairs * p.hkv, ktiles = (p.len_k + kTileKeys - 1) / kTileKeys;
   int ranks = 1;
-  while (ranks < kMaxCluster && units * ranks * 2 <= sm_count() && ktiles >= ranks * 8) ranks *= 2;
+  while (ranks < kMaxCluster && units * ranks <= sm_count() && ktiles >= ranks * 8) ranks *= 2;
   const bool bf16 = dtype == HFAN_BFLOAT16;
   if (p.d == 128) return bf16 ? run_norm<128, true>(p, c, ranks, flags, s) : run_norm<128, false>(p, c, ranks, flags, s);
   return bf16 ? run_norm<64, true>(p, c, ranks, flags, s) : run_norm<64, false>(p, c, ranks, flags, s);

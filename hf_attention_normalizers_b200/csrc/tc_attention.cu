@@ -224,14 +224,6 @@ __device__ __noinline__ Cand buffer_compact(float* buf, uint16_t* ibuf, int row,
   return c;
 }
 
-// Two 16-bit values (low half first in memory) -> packed f32x2.
-template <bool BF16>
-__device__ __forceinline__ uint64_t unpack2(uint32_t x) {
-  if (BF16) return f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
-  return f2_pack(f.x, f.y);
-}
-
 // ------------------------------------------------------------------ kernel
 template <int HD, bool BF16, int NORM, bool DROP>
 __global__ void __launch_bounds__(Roles<HD, 2>::THREADS, 1)

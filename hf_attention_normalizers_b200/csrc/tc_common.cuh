@@ -91,6 +91,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// Two 16-bit values (low half first in memory) -> packed f32x2.
+template <bool BF16>
+__device__ __forceinline__ uint64_t unpack2(uint32_t x) {
+  if (BF16) return f2_pack(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return f2_pack(f.x, f.y);
+}
+
 // P (or dS) row r of a 128 x 128 16-bit tile -> shared memory, K-major with
 // 128-byte swizzle: two 64-column halves kHalf apart; 16-byte chunk c of row
 // r sits at chunk position c ^ (r & 7).  `pk` holds the row as 64 packed pairs.

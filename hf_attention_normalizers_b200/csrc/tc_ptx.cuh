@@ -92,6 +92,47 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// ---------------------------------------------------------------- shared memory
+// Explicit shared-space accesses: through a generic pointer a scattered store
+// costs a warp about 45 cycles of issue, these a few.
+__device__ __forceinline__ void sts_f32_if(bool on, uint32_t addr, float v) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p st.shared.f32 [%1], %2;\n\t}" ::"r"((uint32_t)on),
+               "r"(addr), "f"(v)
+               : "memory");
+}
+__device__ __forceinline__ void sts_u16_if(bool on, uint32_t addr, uint32_t v) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p st.shared.u16 [%1], %2;\n\t}" ::"r"((uint32_t)on),
+               "r"(addr), "h"((uint16_t)v)
+               : "memory");
+}
+// When x > gate: stores z and the low half of id at za / ia and moves both on.
+__device__ __forceinline__ void push_if_above(float x, float gate, float z, uint32_t id, uint32_t& za, uint32_t& ia,
+                                              uint32_t zstep, uint32_t istep) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.gt.f32 p, %2, %3;\n\t"
+      "@p st.shared.f32 [%0], %4;\n\t"
+      "@p st.shared.u16 [%1], %5;\n\t"
+      "@p add.u32 %0, %0, %6;\n\t"
+      "@p add.u32 %1, %1, %7;\n\t}"
+      : "+r"(za), "+r"(ia)
+      : "f"(x), "f"(gate), "f"(z), "r"(id), "r"(zstep), "r"(istep)
+      : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_b32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
 // ---------------------------------------------------------------- cluster
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
