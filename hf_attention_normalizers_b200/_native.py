@@ -113,9 +113,9 @@ SIGNATURES = {
     "hfan_paged_decode_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PagedDesc)]),
     "hfan_paged_decode": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _T, _T, _T, _T, _P, _P, ctypes.c_int64, _P]),
     "hfan_paged_decode_static": (ctypes.c_int, [ctypes.POINTER(PagedDesc), _T, _T, _T, _T, _P, _P]),
-    "hfan_paged_chunk_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ChunkDesc)]),
-    "hfan_paged_chunk_fwd": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _T, _T, _P, _P, ctypes.c_int64, _P]),
-    "hfan_paged_key_weights": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _P, _P, ctypes.c_int64, _P]),
+    "hfan_paged_chunk_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ChunkDesc), ctypes.c_int32]),
+    "hfan_paged_chunk_fwd": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _T, _T, _P, _P, ctypes.c_int64, _P,
+                                            ctypes.c_int64, _P]),
     "hfan_paged_append": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _T, _T, _P, ctypes.c_int64, _P]),
     "hfan_paged_evict": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _T, _T, _P, ctypes.c_int64, ctypes.c_int32,
                                         ctypes.c_int32, _P, _P, _P]),

@@ -489,51 +489,38 @@ int hfan_paged_decode_static(const hfan_paged_desc* desc, hfan_tensor q, hfan_te
   return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_decode_static");
 }
 
-int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc) {
+int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc, int32_t with_key_weights) {
   AttnParams p;
   std::memset(&p, 0, sizeof(p));
   if (fill_chunk_rows(desc, p) != HFAN_OK) return -1;
-  return chunk_tc_workspace(p);
+  return chunk_tc_workspace(p, with_key_weights != 0);
 }
 
 int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, hfan_tensor value_cache,
-                         hfan_tensor o, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+                         hfan_tensor o, float* stats, float* key_weights, int64_t ld_weights, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
   AttnParams p = base_params(q, key_cache, value_cache, o);
   int rc = fill_chunk_rows(desc, p);
   if (rc != HFAN_OK) return rc;
+  if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
   if (desc->total_q == 0 || desc->max_len_q == 0) return HFAN_OK;
   if (stats == nullptr) return fail(HFAN_ERR_INVALID, "stats buffer is required");
   p.stats = stats;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (chunk_tc_supported(desc->dtype, p)) {
-    const int64_t need = chunk_tc_workspace(p);
+    const int64_t need = chunk_tc_workspace(p, key_weights != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
       return fail(HFAN_ERR_INVALID, "paged chunk: workspace of %lld bytes required", (long long)need);
     if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
       return fail(HFAN_ERR_INVALID, "paged chunk: workspace must be 256-byte aligned");
-    e = chunk_tc_fwd(desc->dtype, p, workspace, s);
+    e = chunk_tc_fwd(desc->dtype, p, key_weights, ld_weights, workspace, s);
   } else {
     e = simt_attention_fwd(desc->dtype, p, desc->max_len_q, s);
+    if (e == cudaSuccess && key_weights != nullptr && desc->max_len_k > 0)
+      e = serving_key_weights(desc->dtype, p, key_weights, ld_weights, s);
   }
   return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_chunk_fwd");
-}
-
-int hfan_paged_key_weights(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, const float* stats,
-                           float* key_weights, int64_t ld_weights, void* stream) {
-  AttnParams p = base_params(q, key_cache, key_cache, q);
-  int rc = fill_chunk_rows(desc, p);
-  if (rc != HFAN_OK) return rc;
-  if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
-  if (desc->total_q == 0 || desc->max_len_q == 0 || desc->max_len_k == 0) return HFAN_OK;
-  if (stats == nullptr || key_weights == nullptr)
-    return fail(HFAN_ERR_INVALID, "stats and key_weights buffers are required");
-  p.stats = const_cast<float*>(stats);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = chunk_tc_weights_supported(desc->dtype, p)
-                      ? chunk_tc_weights(desc->dtype, p, key_weights, ld_weights, s)
-                      : serving_key_weights(desc->dtype, p, key_weights, ld_weights, s);
-  return e == cudaSuccess ? HFAN_OK : cuda_fail(e, "hfan_paged_key_weights");
 }
 
 int hfan_paged_append(const hfan_chunk_desc* desc, hfan_tensor k, hfan_tensor v, hfan_tensor key_cache,

@@ -128,4 +128,11 @@ inline bool make_page_map(CUtensorMap* m, const void* cache, int64_t st, int64_t
 // unit whose flag it leaves 0 (flags [pairs][hkv]).
 cudaError_t chunk_sparse_scan(int dtype, const AttnParams& p, const ChunkPlan& c, int* flags, cudaStream_t s);
 
+// softmax1 with at most 32 packed rows a sequence (paged_few_tc.cu); adds to
+// the key weights kw [hkv][ldw] when it is given.
+bool chunk_few_applies(const AttnParams& p, const ChunkPlan& c, bool weights);
+int64_t chunk_few_workspace(const AttnParams& p, const ChunkPlan& c, bool weights);
+cudaError_t chunk_few_fwd(int dtype, const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw, void* workspace,
+                          cudaStream_t s);
+
 }  // namespace hfan

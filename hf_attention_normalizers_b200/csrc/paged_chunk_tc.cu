@@ -716,7 +716,7 @@ cudaError_t weights_t(const AttnParams& p, const ChunkPlan& c, float* kw, int64_
   return cudaGetLastError();
 }
 
-// F<HD, BF16, NORM>::run(args...) for the request's types.
+// fn<HD, BF16, NORM>(args...) for the request's types.
 #define HFAN_CHUNK_DISPATCH(fn, ...)                                                                             \
   const bool bf16 = dtype == HFAN_BFLOAT16;                                                                      \
   switch (p.norm) {                                                                                              \
@@ -748,18 +748,24 @@ bool chunk_tc_supported(int dtype, const AttnParams& p) {
          stride_ok(p.v_sh) && p.o_st % 8 == 0 && p.o_sh % 8 == 0;
 }
 
-int64_t chunk_tc_workspace(const AttnParams& p) { return ws_layout(p, plan_of(p)).total; }
-
-cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, void* workspace, cudaStream_t s) {
+int64_t chunk_tc_workspace(const AttnParams& p, bool weights) {
   const ChunkPlan c = plan_of(p);
+  return chunk_few_applies(p, c, weights) ? chunk_few_workspace(p, c, weights) : ws_layout(p, c).total;
+}
+
+static cudaError_t dense_fwd(int dtype, const AttnParams& p, const ChunkPlan& c, void* workspace, cudaStream_t s) {
   HFAN_CHUNK_DISPATCH(fwd_t, p, c, workspace, s)
 }
 
-bool chunk_tc_weights_supported(int dtype, const AttnParams& p) { return keys_supported(dtype, p); }
-
-cudaError_t chunk_tc_weights(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s) {
-  const ChunkPlan c = plan_of(p);
+static cudaError_t dense_weights(int dtype, const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw, cudaStream_t s) {
   HFAN_CHUNK_DISPATCH(weights_t, p, c, kw, ldw, s)
+}
+
+cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, float* kw, int64_t ldw, void* workspace, cudaStream_t s) {
+  const ChunkPlan c = plan_of(p);
+  if (chunk_few_applies(p, c, kw != nullptr)) return chunk_few_fwd(dtype, p, c, kw, ldw, workspace, s);
+  const cudaError_t e = dense_fwd(dtype, p, c, workspace, s);
+  return e != cudaSuccess || kw == nullptr ? e : dense_weights(dtype, p, c, kw, ldw, s);
 }
 
 }  // namespace hfan

@@ -17,13 +17,11 @@ cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw
 // kw[kvh][slot] += sum of p over the chunk's rows of the KV group (p.stats: what the forward saved).
 cudaError_t serving_key_weights(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s);
 
-// Tensor-core forms (paged_chunk_tc.cu) of the chunk attention and the key
-// weights.  The workspace size depends on sizes alone, so it may be asked for
-// before the tensors are known.
+// Tensor-core form (paged_chunk_tc.cu) of the chunk attention and, when kw is
+// given, the key weights.  The workspace size depends on sizes alone, so it may
+// be asked for before the tensors are known.
 bool chunk_tc_supported(int dtype, const AttnParams& p);
-int64_t chunk_tc_workspace(const AttnParams& p);
-cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, void* workspace, cudaStream_t s);
-bool chunk_tc_weights_supported(int dtype, const AttnParams& p);
-cudaError_t chunk_tc_weights(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s);
+int64_t chunk_tc_workspace(const AttnParams& p, bool weights);
+cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, float* kw, int64_t ldw, void* workspace, cudaStream_t s);
 
 }  // namespace hfan

@@ -1,0 +1,224 @@
+// How the tensor-core chunk kernels share the work of a ragged batch.
+//
+// A unit is a group of `per` tokens of one sequence under one KV head; its work
+// is its key tiles.  All units' tiles, in (sequence, KV head, group) order,
+// form one line that is cut into equal stretches, one per CTA: every SM gets
+// the same number of tiles however ragged the lengths are.  A stretch may start
+// and end inside a unit, so a CTA has at most two partial results, its first
+// piece and its last; combine_kernel joins the pieces of a unit.
+#pragma once
+
+#include "paged_chunk.cuh"
+
+namespace hfan {
+
+// What the pieces of a unit leave for combine_kernel.
+struct PieceWs {
+  float* o;    // [2 * ctas][rows of a unit][D] unscaled O of a partial piece
+  float2* ml;  // [2 * ctas][rows of a unit] (reference m, sum l)
+  int4* info;  // [total_q][hkv] (first tile of the unit on the line, its tiles, first row of the token, tiles of a CTA)
+  int rows;    // rows of a unit
+  int ctas;
+};
+
+struct Unit {
+  int b, kvh, tok0, ntok;  // tokens [tok0, tok0 + ntok) of sequence b
+  int tiles;               // key tiles it sees (at least one, which may be masked altogether)
+  Geometry g;
+};
+
+struct Piece {
+  int kt0, nt;  // key tiles [kt0, kt0 + nt) of the unit
+  int u0;       // the unit's first tile on the line
+  int slot;     // partial results
+  bool whole;
+};
+
+class Walk {
+ public:
+  Unit u;
+  Piece piece;
+  int quota;  // tiles of a CTA
+
+  // Whole-warp call: finds the start of this CTA's stretch.
+  __device__ __forceinline__ Walk(const AttnParams& p, int per) : p_(p), per_(per) {
+    const int lane = threadIdx.x & 31;
+    int total = 0;
+    for (int base = 0; base < p.batch; base += 32)
+      total += __reduce_add_sync(0xffffffffu, base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0);
+    quota = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 2);
+    at_ = (int)blockIdx.x * quota;
+    end_ = min(at_ + quota, total);
+    if (at_ >= end_) return;
+    int before = 0;
+    for (int base = 0;; base += 32) {
+      const int w = base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0;
+      int inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > at_);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        enter(base + l);
+        int off = at_ - before - __shfl_sync(0xffffffffu, inc - w, l);
+        const int one = __shfl_sync(0xffffffffu, w, l) / p.hkv;
+        u.kvh = off / one;
+        off -= u.kvh * one;
+        group_ = 0;
+        load_group();
+        while (off >= u.tiles) {
+          off -= u.tiles;
+          ++group_;
+          load_group();
+        }
+        u0_ = at_ - off;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+
+  // Moves to the next piece of the stretch; false when it is done.
+  __device__ __forceinline__ bool next() {
+    if (at_ >= end_) return false;
+    if (at_ >= u0_ + u.tiles) {  // the next unit
+      u0_ = at_;
+      ++group_;
+      if (group_ * per_ >= u.g.q_len) {
+        group_ = 0;
+        if (++u.kvh == p_.hkv) {
+          u.kvh = 0;
+          int b = u.b, s;
+          do ++b;
+          while (chunk_tokens(p_, b, &s) == 0);  // (the line has tiles left, so some sequence follows)
+          enter(b);
+        }
+      }
+      load_group();
+    }
+    piece.kt0 = at_ - u0_;
+    piece.nt = min(u.tiles - piece.kt0, end_ - at_);
+    piece.u0 = u0_;
+    piece.whole = piece.nt == u.tiles;
+    piece.slot = 2 * (int)blockIdx.x + (at_ == (int)blockIdx.x * quota ? 0 : 1);
+    at_ += piece.nt;
+    return true;
+  }
+
+ private:
+  __device__ __forceinline__ int group_tiles(int n, int k_len, int j) const {
+    const int end = min((j + 1) * per_, n);  // tokens up to here see keys up to end + (k_len - n)
+    const int k_hi = p_.causal ? min(k_len, end + k_len - n) : k_len;
+    return max((k_hi + kTileKeys - 1) / kTileKeys, 1);
+  }
+  __device__ __forceinline__ int sequence_tiles(int b) const {
+    int s;
+    const int n = chunk_tokens(p_, b, &s);
+    const int k_len = min(max(p_.seq_lens[b], 0), p_.len_k);
+    int sum = 0;
+    for (int j = 0; j * per_ < n; ++j) sum += group_tiles(n, k_len, j);
+    return sum;
+  }
+  __device__ __forceinline__ void enter(int b) {
+    u.b = b;
+    u.g = geometry(p_, b);
+  }
+  __device__ __forceinline__ void load_group() {
+    u.tok0 = group_ * per_;
+    u.ntok = min(per_, u.g.q_len - u.tok0);
+    u.tiles = group_tiles(u.g.q_len, u.g.k_len, group_);
+  }
+
+  const AttnParams& p_;
+  int per_, at_, end_, u0_, group_;
+};
+
+// Joins the pieces of split units: one block per (token, KV head) and its G rows.
+template <int HD, typename T, int NORM>
+__global__ void __launch_bounds__(128) combine_pieces_kernel(const AttnParams p, const PieceWs ws, int group) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the pieces are still being computed
+  const int tok = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
+  const int4 f = ws.info[blockIdx.x];
+  // (a token that no sequence owns has no info: kept inside the workspace)
+  const int quota = max(f.w, 1), first = min(max(f.x / quota, 0), ws.ctas - 1);
+  const int last = min(max((f.x + f.y - 1) / quota, first), ws.ctas - 1);
+  if (last == first) return;
+  const int head = 2 * first + (f.x == first * quota ? 0 : 1);  // slot of the unit's first piece; the others lead their CTA
+  constexpr int LPR = HD / 4;                                   // lanes of a row
+  for (int g = threadIdx.x / LPR; g < group; g += 128 / LPR) {
+    const int d = (threadIdx.x % LPR) * 4, row = min(max(f.z, 0), ws.rows - group) + g;
+    float m = 0.f, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (NORM == HFAN_SOFTMAX1)
+      for (int c = first; c <= last; ++c) m = fmaxf(m, ws.ml[(int64_t)(c == first ? head : 2 * c) * ws.rows + row].x);
+#pragma unroll 4
+    for (int c = first; c <= last; ++c) {
+      const int64_t at = (int64_t)(c == first ? head : 2 * c) * ws.rows + row;
+      const float4 x = *reinterpret_cast<const float4*>(ws.o + at * HD + d);
+      float s = 1.f;
+      if (NORM == HFAN_SOFTMAX1) {
+        const float2 ml = ws.ml[at];
+        s = exp2f(ml.x - m);
+        l += ml.y * s;
+      }
+      acc.x = fmaf(s, x.x, acc.x);
+      acc.y = fmaf(s, x.y, acc.y);
+      acc.z = fmaf(s, x.z, acc.z);
+      acc.w = fmaf(s, x.w, acc.w);
+    }
+    const int h = kvh * group + g;
+    float inv = 1.f;
+    if (NORM == HFAN_SOFTMAX1) {
+      l += exp2f(-m);  // the implicit zero logit
+      inv = 1.f / l;
+      if (d == 0) {
+        p.stats[(int64_t)h * p.rows_total + tok] = m;
+        p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = l;
+      }
+    }
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    uint2 y;
+    y.x = tc::pack2<BF16>(acc.x * inv, acc.y * inv);
+    y.y = tc::pack2<BF16>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (int64_t)tok * p.o_st + (int64_t)h * p.o_sh + d) = y;
+  }
+}
+
+struct PieceLayout {
+  int64_t o, ml, info, total;
+};
+inline PieceLayout piece_layout(const AttnParams& p, int ctas, int rows) {
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  PieceLayout w;
+  w.o = 0;
+  w.ml = up((int64_t)2 * ctas * rows * p.d * 4);
+  w.info = w.ml + up((int64_t)2 * ctas * rows * 8);
+  w.total = w.info + up((int64_t)p.rows_total * p.hkv * 16);
+  return w;
+}
+inline PieceWs piece_ws(const AttnParams& p, int ctas, int rows, void* workspace) {
+  const PieceLayout w = piece_layout(p, ctas, rows);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  return PieceWs{reinterpret_cast<float*>(base + w.o), reinterpret_cast<float2*>(base + w.ml),
+                 reinterpret_cast<int4*>(base + w.info), rows, ctas};
+}
+
+// A launch that may begin while its predecessor on the stream still runs (it waits inside).
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace hfan

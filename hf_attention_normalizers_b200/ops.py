@@ -544,18 +544,14 @@ def launch_paged_chunk_fwd(q: Tensor, key_cache: Tensor, value_cache: Tensor, bl
     stats = torch.empty((2, hq, total), dtype=torch.float32, device=q.device)
     desc = _Desc(dtype_id(q), normalizer, batch, hq, hkv, d, total, max_q, page_size, cols, max_k, slots, bt.data_ptr(),
                  cu.data_ptr(), sl.data_ptr(), scale, causal)
-    lib, ref, qv, kv, stream = N.lib(), ctypes.byref(desc), _rows3(q), _rows3(key_cache), _raw_stream(q.get_device())
-    nbytes = lib.hfan_paged_chunk_workspace_bytes(ref)
+    kw, ld = (None, 0) if key_weights is None else (key_weights.data_ptr(), key_weights.stride(0))
+    lib, ref = N.lib(), ctypes.byref(desc)
+    nbytes = lib.hfan_paged_chunk_workspace_bytes(ref, kw is not None)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    sp = stats.data_ptr()
-    rc = lib.hfan_paged_chunk_fwd(ref, qv, kv, _rows3(value_cache), _rows3(o), sp, None if ws is None else ws.data_ptr(),
-                                  nbytes if nbytes > 0 else 0, stream)
+    rc = lib.hfan_paged_chunk_fwd(ref, _rows3(q), _rows3(key_cache), _rows3(value_cache), _rows3(o), stats.data_ptr(), kw, ld,
+                                  None if ws is None else ws.data_ptr(), max(nbytes, 0), _raw_stream(q.get_device()))
     if rc:
         N.check(rc, "hfan_paged_chunk_fwd")
-    if key_weights is not None:
-        rc = lib.hfan_paged_key_weights(ref, qv, kv, sp, key_weights.data_ptr(), key_weights.stride(0), stream)
-        if rc:
-            N.check(rc, "hfan_paged_key_weights")
     return o, stats
 
 

@@ -265,20 +265,17 @@ typedef struct hfan_chunk_desc {
 } hfan_chunk_desc;
 
 /* Attention of the new tokens over the cached context.  q, o: packed views.
- * stats: float32 [2, heads_q, total_q] as for hfan_attn_fwd.  workspace: device
- * scratch of hfan_paged_chunk_workspace_bytes(desc) bytes, 256-byte aligned
- * (NULL when that is 0). */
-int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc);
+ * stats: float32 [2, heads_q, total_q] as for hfan_attn_fwd.  With key_weights
+ * (or NULL), key_weights[kvh][slot] += the sum over the group's query heads and
+ * the new tokens of their probabilities on that key: a slot that is in one
+ * sequence's pages is added to once (the same bits on every run), slots of
+ * pages that several sequences share once per sequence, in no fixed order.
+ * workspace: device scratch of hfan_paged_chunk_workspace_bytes(desc,
+ * key_weights != NULL) bytes, 256-byte aligned (NULL when that is 0). */
+int64_t hfan_paged_chunk_workspace_bytes(const hfan_chunk_desc* desc, int32_t with_key_weights);
 int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, hfan_tensor value_cache,
-                         hfan_tensor o, float* stats, void* workspace, int64_t workspace_bytes, void* stream);
-
-/* key_weights[kvh][slot] += the sum over the group's query heads and the new
- * tokens of their probabilities on that key; q and stats as given to and
- * written by hfan_paged_chunk_fwd.  A slot that is in one sequence's pages is
- * added to once (the same bits on every run); slots of pages that several
- * sequences share are added to once per sequence, in no fixed order. */
-int hfan_paged_key_weights(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor key_cache, const float* stats,
-                           float* key_weights, int64_t ld_weights, void* stream);
+                         hfan_tensor o, float* stats, float* key_weights, int64_t ld_weights, void* workspace,
+                         int64_t workspace_bytes, void* stream);
 
 /* Writes the new tokens' K/V rows to their slots and zeroes the slots' key
  * weights (key_weights may be NULL).  normalizer, heads_q and scale are ignored. */

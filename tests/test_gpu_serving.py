@@ -225,6 +225,29 @@ def test_peaked_and_flat_rows_share_a_tile():
         _chunk_case(b, norm)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [2, 5], [70, 40]])
+@pytest.mark.parametrize("norm", NORMS)
+def test_scores_that_grow_along_the_keys(norm, new):
+    """Row maxima that rise by far more than 2^8 from one key tile to the next, and from one part of the keys to another."""
+    b = Batch(new, [900, 3000], seed=18, hkv=1)
+    for r in b.rows:
+        b.key_cache[r] *= torch.linspace(0.1, 25.0, len(r)).to(b.dtype)[:, None, None]
+    b.d_key = b.key_cache.cuda()
+    _chunk_case(b, norm)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,new", [(1, [1, 32, 0, 7]), (8, [4, 1, 2]), (3, [5, 1]), (32, [1, 1]), (5, [3, 1, 0, 1])])
+def test_few_rows(group, new, dim):
+    lens = [513, 100, 1300, 129, 64][:len(new)]
+    _chunk_case(Batch(new, lens, seed=19, group=group, hkv=2, dim=dim, gain=2.0), "softmax1")
+
+
+def test_wrong_hint_of_the_longest_chunk():
+    """A hint smaller than a sequence's chunk only sets the tile size."""
+    _chunk_case(Batch([40, 3], [300, 130], seed=20), "softmax1", max_seqlen_q=2)
+
+
 def test_same_bits_on_every_run():
     for norm in NORMS:
         outs = []

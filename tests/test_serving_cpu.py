@@ -65,11 +65,10 @@ def _desc(**kw):
 def test_requests_are_refused_on_the_host(kw, msg):
     lib, t = N.lib(), N.HfanTensor(None, 0, 0, 0)
     one = ctypes.c_void_p(1)
-    assert lib.hfan_paged_chunk_fwd(ctypes.byref(_desc(**kw)), t, t, t, t, one, None, 0, None) == 1
+    assert lib.hfan_paged_chunk_fwd(ctypes.byref(_desc(**kw)), t, t, t, t, one, None, 0, None, 0, None) == 1
     assert msg in lib.hfan_last_error().decode()
-    assert lib.hfan_paged_key_weights(ctypes.byref(_desc(**kw)), t, t, one, one, 64, None) == 1
     assert lib.hfan_paged_append(ctypes.byref(_desc(**kw)), t, t, t, t, None, 0, None) == 1
-    assert lib.hfan_paged_chunk_workspace_bytes(ctypes.byref(_desc(**kw))) == -1
+    assert lib.hfan_paged_chunk_workspace_bytes(ctypes.byref(_desc(**kw)), 0) == -1
 
 
 @pytest.mark.parametrize("budget,recent,ld,msg", [(0, 0, 64, "budget"), (4, -1, 64, "recent"), (4, 0, 63, "every cache slot")])
