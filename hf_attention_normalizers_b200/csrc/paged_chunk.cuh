@@ -21,9 +21,7 @@ struct ChunkPlan {
   int group;     // query heads per KV head
   int tpb;       // tokens per tile
   int box_rows;  // rows of one TMA box of a page: a power of two that divides the page size, 8 .. 128
-  int splits;    // parts of the key axis (grid z)
-  int span;      // key tiles per part
-  int pairs;     // upper bound of the tile pairs of all sequences (grid x)
+  int pairs;     // upper bound of the tile pairs of all sequences
 };
 
 // Tokens of sequence b and the first of them, clamped as geometry() does.

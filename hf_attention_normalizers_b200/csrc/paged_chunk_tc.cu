@@ -2,15 +2,16 @@
 // tensor cores (16-bit inputs, head_dim 64 / 128, pages of a multiple of 8
 // tokens, positive scale).
 //
-// One CTA takes two tiles of 128 packed (token, head) rows of one sequence and
-// KV head over one part of its keys, in tiles of 128 keys that TMA fetches
-// straight from the pages (one box per page or per 128 rows of it):
+// A unit of work is two tiles of 128 packed (token, head) rows of one sequence
+// and KV head; a CTA takes pieces of units (paged_walk.cuh) in tiles of 128
+// keys that TMA fetches straight from the pages (one box per page or per 128
+// rows of it):
 //
 //   warps 0-3, 4-7  row warps of tile 0 / 1: thread = TMEM lane = row.  A
 //                   thread reads its whole S row, so the running maximum and
 //                   sum need no exchange, and writes P over S as packed
 //                   16-bit pairs (the A operand of P V).
-//   warp 8          producer: Q once, then K0 V0 K1 V1 ... through one ring.
+//   warp 8          producer: Q of a piece, then K0 V0 K1 V1 ... through one ring.
 //   warps 9, 10     MMA issuers of tile 0 / 1: S = Q K^T, then O += P V, then
 //                   the next S over the P just consumed.
 //
@@ -21,13 +22,14 @@
 // 2^8.  P V of tile t is done before S of tile t + 1 (same issuer), so the row
 // warps that hold S of t + 1 may rescale O without another wait.
 //
-// With few rows the key axis is split over grid z; the parts leave unscaled O
-// with (m, l) in the workspace and combine_kernel joins them.
+// sparsemax / entmax15 come here with their thresholds known, for the units
+// that the scan (paged_chunk_sparse.cu) could not serve from its buffers.
 #include <cuda.h>
 
 #include "common.cuh"
 #include "paged_chunk.cuh"
 #include "paged_serving.cuh"
+#include "paged_walk.cuh"
 #include "params.cuh"
 #include "tc_common.cuh"
 #include "tc_ptx.cuh"
@@ -44,13 +46,14 @@ constexpr int kRowRegs = 224, kHelperRegs = 56;
 static_assert(256 * kRowRegs + 128 * kHelperRegs <= 384 * 168, "more registers than the block was launched with");
 constexpr int kMaxRing = 8;
 constexpr float kRescale = 8.f;
+constexpr int kUnitRows = 2 * kTileRows;
 
 template <int HD>
 constexpr int chunk_ring() { return HD == 128 ? 5 : 8; }
 
 struct ChunkBars {
-  uint64_t q_full, full[kMaxRing], empty[kMaxRing];
-  uint64_t s_full[2], p_full[2], o_full[2], drain[2];
+  uint64_t q_full, q_empty, full[kMaxRing], empty[kMaxRing];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2], drain[2];
 };
 struct ChunkCtl {
   uint32_t tmem;
@@ -67,25 +70,55 @@ struct ChunkLayout {
   static constexpr uint32_t TOTAL = CTL + sizeof(ChunkCtl) + 1024;
 };
 
-// Partial results of the split key axis.
-struct ChunkWs {
-  float* o;    // [splits][total_q * hq][D]
-  float2* ml;  // [splits][total_q * hq]
-  int* parts;  // [total_q * hq] parts that the row has (1: already final)
-  int* flags;  // sparse: [pairs][hkv], 0 where the scan has written the output
-};
-
 __device__ __forceinline__ void fail(const AttnParams& p, ChunkCtl* ctl) {
   ctl->abort = 1;
   if (p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevWaitTimeout);
 }
 
+// The sparse normalizers' source of work: the unit of the block's grid
+// coordinates, when the scan has left its output to this kernel.
+class FlaggedUnit {
+ public:
+  Unit u;
+  Piece piece;
+  static constexpr int quota = 1;
+  __device__ __forceinline__ FlaggedUnit(const AttnParams& p, int per, const int* flags) {
+    int group;
+    left_ = find_group(p, per, blockIdx.x, &u.b, &group) && flags[blockIdx.x * p.hkv + blockIdx.y] != 0;
+    if (!left_) return;
+    u.g = geometry(p, u.b);
+    u.kvh = blockIdx.y;
+    u.tok0 = group * per;
+    u.ntok = min(per, u.g.q_len - u.tok0);
+    const int k_hi = p.causal ? min(u.g.k_len, u.tok0 + u.ntok + u.g.shift) : u.g.k_len;
+    u.tiles = max((k_hi + kTileKeys - 1) / kTileKeys, 1);
+    piece = Piece{0, u.tiles, 0, 0, true};
+  }
+  __device__ __forceinline__ bool any() const { return left_; }
+  __device__ __forceinline__ bool next() {
+    const bool r = left_;
+    left_ = false;
+    return r;
+  }
+
+ private:
+  bool left_;
+};
+
+class Stretch : public Walk {
+ public:
+  __device__ __forceinline__ Stretch(const AttnParams& p, int per, const int*) : Walk(p, per) {}
+  __device__ __forceinline__ bool any() const { return true; }
+};
+
 template <int HD, bool BF16, int NORM>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const AttnParams p, const ChunkPlan c, const ChunkWs ws) {
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p,
+                     const __grid_constant__ ChunkPlan c, const __grid_constant__ PieceWs ws, const int* flags) {
   using L = ChunkLayout<HD>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  using Source = typename std::conditional<NORM == HFAN_SOFTMAX1, Stretch, FlaggedUnit>::type;
   constexpr int NH = L::NH, NS = L::NS;
   constexpr uint32_t IDESC_QK = idesc_f16(BF16, 128, 128, false, false);
   constexpr uint32_t IDESC_PV = idesc_f16(BF16, 128, HD, false, true);
@@ -96,34 +129,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   ChunkCtl* ctl = reinterpret_cast<ChunkCtl*>(smem + L::CTL);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  int b, pair;
-  if (!find_group(p, 2 * c.tpb, blockIdx.x, &b, &pair)) return;
-  const Geometry g = geometry(p, b);
-  const int kvh = blockIdx.y, split = blockIdx.z;
-  if (NORM != HFAN_SOFTMAX1 && ws.flags[blockIdx.x * p.hkv + kvh] == 0) return;
-  const int tok0 = pair * 2 * c.tpb, ntok = min(2 * c.tpb, g.q_len - tok0);
-  const int nact = ntok > c.tpb ? 2 : 1;  // tiles with rows
-  const int k_hi = p.causal ? min(g.k_len, tok0 + ntok + g.shift) : g.k_len;
-  const int n_all = k_hi > 0 ? (k_hi + kTileKeys - 1) / kTileKeys : 0;
-  const int parts = max(1, (n_all + c.span - 1) / c.span);
-  if (split >= parts) return;
-  const int kt0 = split * c.span, nt = min(c.span, n_all - kt0);
-
+  allow_dependents();
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 2);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], nact);
+      mbar_init(&bars->empty[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s], 4);
+      mbar_init(&bars->p_full[s][0], 4);
+      mbar_init(&bars->p_full[s][1], 4);
       mbar_init(&bars->o_full[s], 1);
+      mbar_init(&bars->o_empty[s], 4);
       mbar_init(&bars->drain[s], 1);
     }
     ctl->abort = ctl->never = 0;
     fence_barrier_init();
   }
+  Source src(p, 2 * c.tpb, flags);
+  if (!src.any()) return;  // nothing was left to this block
   if (warp == 8) tmem_alloc(&ctl->tmem, 512);
   tc_fence_before();
   __syncthreads();
@@ -132,135 +163,171 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   volatile int* abort_flag = &ctl->abort;
 
   if (warp >= 8) {
-  set_max_regs<kHelperRegs, false>();
-  if (warp == 8) {
-    // ------------------------------------------------------------ producer
-    if (nt > 0) {
-      if (lane == 0) {
-        prefetch_tmap(&tm_k);
-        prefetch_tmap(&tm_v);
-        mbar_arrive_expect_tx(&bars->q_full, nact * NH * c.tpb * c.group * 128);
-        for (int q = 0; q < nact; ++q)
-          for (int hh = 0; hh < NH; ++hh)
-            tma_load_4d(smem + q * L::TILE + hh * kHalf, &tm_q, &bars->q_full, 64 * hh, kvh * c.group,
-                        g.q_start + tok0 + q * c.tpb, 0);
-      }
+    set_max_regs<kHelperRegs, false>();
+    if (warp == 8) {
+      // ---------------------------------------------------------- producer
       bool ok = true;
-      int row = tile_box_row(p, c, b, g.k_len, kt0);
-      int st = 0, ph = 1;
-      int issued = 0;
-      for (int t = 0; t < nt && ok; ++t) {
-        const int next = t + 1 < nt ? tile_box_row(p, c, b, g.k_len, kt0 + t + 1) : -1;
-#pragma unroll
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          if (!(ok = wait_warp(&bars->empty[st], ph, abort_flag))) break;
-          load_key_tile_tma<NH>(smem + L::RING + st * L::TILE, kv ? &tm_v : &tm_k, &bars->full[st], row, c.box_rows, kvh);
-          ++issued;
-          if (++st == NS) {
-            st = 0;
-            ph ^= 1;
-          }
-        }
-        row = next;
-      }
-      if (!ok) {
+      int st = 0, ph = 1, issued = 0, pieces = 0;
+      while (ok && src.next()) {
+        const Unit& u = src.u;
+        const int nact = u.ntok > c.tpb ? 2 : 1;  // tiles with rows
+        int row = tile_box_row(p, c, u.b, u.g.k_len, src.piece.kt0);
+        if (!(ok = wait_warp(&bars->q_empty, (pieces & 1) ^ 1, abort_flag))) break;
         if (lane == 0) {
-          fail(p, ctl);
-          // its own copies land before the CTA leaves
-          mbar_wait(&bars->q_full, 0, &ctl->never);
-          for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&bars->full[i % NS], (i / NS) & 1, &ctl->never);
+          mbar_arrive_expect_tx(&bars->q_full, nact * NH * c.tpb * c.group * 128);
+          for (int q = 0; q < nact; ++q)
+            for (int hh = 0; hh < NH; ++hh)
+              tma_load_4d(smem + q * L::TILE + hh * kHalf, &tm_q, &bars->q_full, 64 * hh, u.kvh * c.group,
+                          u.g.q_start + u.tok0 + q * c.tpb, 0);
         }
-        __syncwarp();
+        ++pieces;
+        for (int t = 0; t < src.piece.nt && ok; ++t) {
+          const int next = t + 1 < src.piece.nt ? tile_box_row(p, c, u.b, u.g.k_len, src.piece.kt0 + t + 1) : -1;
+#pragma unroll
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            if (!(ok = wait_warp(&bars->empty[st], ph, abort_flag))) break;
+            load_key_tile_tma<NH>(smem + L::RING + st * L::TILE, kv ? &tm_v : &tm_k, &bars->full[st], row, c.box_rows, u.kvh);
+            ++issued;
+            if (++st == NS) {
+              st = 0;
+              ph ^= 1;
+            }
+          }
+          row = next;
+        }
       }
-    }
-  } else if (warp < 11) {  // (warp 11 fills the warpgroup)
-    // ------------------------------------------------------------ MMA issuers
-    const int q = warp - 9;
-    if (lane == 0 && q < nact && nt > 0) {
+      if (!ok && lane == 0) {
+        fail(p, ctl);
+        // its own copies land before the CTA leaves
+        if (pieces > 0) mbar_wait(&bars->q_full, (pieces - 1) & 1, &ctl->never);
+        for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&bars->full[i % NS], (i / NS) & 1, &ctl->never);
+      }
+      __syncwarp();
+    } else if (warp < 11) {  // (warp 11 fills the warpgroup)
+      // ---------------------------------------------------------- MMA issuers
+      const int q = warp - 9;
       const uint32_t q_base = smem_u32(smem + q * L::TILE), ring = smem_u32(smem + L::RING);
       const uint32_t s_col = tmem + q * 128, o_col = tmem + 256 + q * 128;
-      bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
-      int st = 0, ph = 0;
+      bool ok = true;
+      int st = 0, ph = 0, it = 0, pieces = 0, mine = 0;  // mine: pieces in which this tile has rows
       auto step = [&]() {
         if (++st == NS) {
           st = 0;
           ph ^= 1;
         }
       };
-      for (int t = 0; t < nt && ok; ++t) {
-        if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
-        tc_fence_after();
+      while (src.next()) {
+        if (lane == 0 && ok) {
+          const int nt = src.piece.nt;
+          ok = mbar_wait(&bars->q_full, pieces & 1, abort_flag);
+          if (q == 1 && src.u.ntok <= c.tpb) {
+            // no rows: the stages are only passed on
+            for (int t = 0; t < 2 * nt && ok; ++t) {
+              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+              mbar_arrive(&bars->empty[st]);
+              step();
+            }
+            mbar_arrive(&bars->q_empty);
+          } else {
+            for (int t = 0; t < nt && ok; ++t, ++it) {
+              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+              tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-          mma_f16_ss(s_col, sw128_desc(q_base + o, 16, 1024), sw128_desc(ring + st * L::TILE + o, 16, 1024), IDESC_QK,
-                     kk > 0);
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+                mma_f16_ss(s_col, sw128_desc(q_base + o, 16, 1024), sw128_desc(ring + st * L::TILE + o, 16, 1024), IDESC_QK,
+                           kk > 0);
+              }
+              mma_commit(&bars->s_full[q]);
+              mma_commit(&bars->empty[st]);
+              if (t + 1 == nt) mma_commit(&bars->q_empty);
+              step();
+              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+              // P comes in halves: its first 64 keys are multiplied while the
+              // row warps exponentiate the others
+              if (t == 0 && !(ok = mbar_wait(&bars->o_empty[q], (mine & 1) ^ 1, abort_flag))) break;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (!(ok = mbar_wait(&bars->p_full[q][half], it & 1, abort_flag))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                  mma_f16_ts(o_col, s_col + kk * 8, sw128_desc(ring + st * L::TILE + kk * 16 * 128, kHalf, 1024), IDESC_PV,
+                             t > 0 || kk > 0);
+              }
+              if (!ok) break;
+              mma_commit(&bars->empty[st]);
+              if (t + 1 == nt) mma_commit(&bars->o_full[q]);
+              step();
+            }
+            ++mine;
+          }
+          ++pieces;
         }
-        mma_commit(&bars->s_full[q]);
-        mma_commit(&bars->empty[st]);
-        step();
-        if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
-        if (!(ok = mbar_wait(&bars->p_full[q], t & 1, abort_flag))) break;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < kTileKeys / 16; ++kk)
-          mma_f16_ts(o_col, s_col + kk * 8, sw128_desc(ring + st * L::TILE + kk * 16 * 128, kHalf, 1024), IDESC_PV,
-                     t > 0 || kk > 0);
-        mma_commit(&bars->empty[st]);
-        if (t + 1 == nt) mma_commit(&bars->o_full[q]);
-        step();
+        __syncwarp();
       }
-      if (!ok) {
+      if (lane == 0 && !ok) {
         fail(p, ctl);
         mma_commit(&bars->drain[q]);
         mbar_wait(&bars->drain[q], 0, &ctl->never);
       }
+      __syncwarp();
     }
-    __syncwarp();
-  }
-  } else if ((warp >> 2) < nact) {
+  } else {
     // ------------------------------------------------------------ row warps
     set_max_regs<kRowRegs, true>();
     const int q = warp >> 2, r = threadIdx.x & 127;
-    const int i = tok0 + q * c.tpb + r / c.group;  // token within the sequence
-    const bool row_ok = r < c.tpb * c.group && i < g.q_len;
-    const int h = kvh * c.group + r % c.group;
+    const int rt = r / c.group, rg = r - rt * c.group;  // token of the tile, head of the group
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_addr + q * 128, o_col = tmem + lane_addr + 256 + q * 128;
-    // visible keys [0, vis)
-    int vis = row_ok ? g.k_len : 0;
-    if (p.causal && row_ok) vis = min(vis, i + g.shift + 1);
-    const bool warp_on = __any_sync(0xffffffffu, vis > 0);
     const float zs = NORM == HFAN_SOFTMAX1 ? p.scale * kLog2e : (NORM == HFAN_SPARSEMAX ? p.scale : 0.5f * p.scale);
-    const int64_t si = row_ok ? stat_index(p, g, h, i) : 0;
-    const int64_t srow = (int64_t)(g.q_start + i) * p.hq + h;
-    float m = 0.f, l = 0.f;
-    if (NORM != HFAN_SOFTMAX1) m = row_ok ? p.stats[si] : kPosInf;  // the threshold
     bool ok = true;
-    int vst = 1 % NS, vph = 0;  // stage of V
-    for (int t = 0; t < nt; ++t) {
-      if (!(ok = wait_warp(&bars->s_full[q], t & 1, abort_flag))) break;
-      tc_fence_after();
-      const int kb = (kt0 + t) * kTileKeys;
-      if (kb + kTileKeys > g.k_len) {
-        // V rows past the sequence hold stale or foreign values: zeroed, since
-        // 0 x NaN would reach O (both tiles' warps write the same zeros)
-        if (!(ok = wait_warp(&bars->full[vst], vph, abort_flag))) break;
-        const int lo = g.k_len - kb;
-        uint8_t* v = smem + L::RING + vst * L::TILE;
-        for (int x = r; x < (kTileKeys - lo) * 8 * NH; x += 128) {
-          const int hh = x / ((kTileKeys - lo) * 8), y = x - hh * (kTileKeys - lo) * 8;
-          *reinterpret_cast<uint4*>(v + hh * kHalf + lo * 128 + y * 16) = make_uint4(0u, 0u, 0u, 0u);
+    int it = 0, mine = 0;
+    int items = 0;  // ring items of the pieces before this one
+    while (src.next()) {
+      const Unit& u = src.u;
+      const Piece& pc = src.piece;
+      const int v0 = items + 1;  // item of the piece's first V tile
+      items += 2 * pc.nt;
+      if (q == 1 && u.ntok <= c.tpb) continue;
+      const int tl = q * c.tpb + rt, i = u.tok0 + tl;  // token of the unit, of the sequence
+      const bool row_ok = rt < c.tpb && tl < u.ntok;
+      const int h = u.kvh * c.group + rg;
+      // visible keys [0, vis)
+      int vis = row_ok ? u.g.k_len : 0;
+      if (p.causal && row_ok) vis = min(vis, i + u.g.shift + 1);
+      const bool warp_on = __any_sync(0xffffffffu, vis > pc.kt0 * kTileKeys);
+      const int64_t si = row_ok ? stat_index(p, u.g, h, i) : 0;
+      float m = 0.f, l = 0.f;
+      if (NORM != HFAN_SOFTMAX1) m = row_ok ? p.stats[si] : kPosInf;  // the threshold
+      for (int t = 0; t < pc.nt; ++t, ++it) {
+        if (ok) ok = wait_warp(&bars->s_full[q], it & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const int kb = (pc.kt0 + t) * kTileKeys;
+        if (kb + kTileKeys > u.g.k_len) {
+          // V rows past the sequence hold stale or foreign values: zeroed, since
+          // 0 x NaN would reach O (both tiles' warps write the same zeros)
+          const int item = v0 + 2 * t, vst = item % NS, lo = max(u.g.k_len - kb, 0);
+          if (!(ok = wait_warp(&bars->full[vst], (item / NS) & 1, abort_flag))) break;
+          uint8_t* v = smem + L::RING + vst * L::TILE;
+          for (int x = r; x < (kTileKeys - lo) * 8 * NH; x += 128) {
+            const int hh = x / ((kTileKeys - lo) * 8), y = x - hh * (kTileKeys - lo) * 8;
+            *reinterpret_cast<uint4*>(v + hh * kHalf + lo * 128 + y * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
-      }
-      vst += 2;
-      if (vst >= NS) {
-        vst -= NS;
-        vph ^= 1;
-      }
-      uint32_t pk[64];
-      if (warp_on) {
+        if (!warp_on) {
+          const uint32_t zero[32] = {};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            tmem_st32(s_col + half * 32, zero);
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&bars->p_full[q][half]);
+          }
+          continue;
+        }
         float s[128];
         {
           uint32_t x[4][32];
@@ -278,64 +345,64 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const uint64_t zs2 = f2_pack(zs, zs);
         if (NORM == HFAN_SOFTMAX1) {
           const float top = max_n<128>(s) * zs;
-          float alpha = 1.f;
-          if (top > m + kRescale) {
-            alpha = exp2f(m - top);
-            m = top;
-            l *= alpha;
-          }
-          if (__any_sync(0xffffffffu, alpha != 1.f) && t > 0) {
+          if (__any_sync(0xffffffffu, top > m + kRescale)) {
+            float alpha = 1.f;
+            if (top > m + kRescale) {
+              alpha = exp2f(m - top);
+              m = top;
+              l *= alpha;
+            }
+            if (t > 0) {
+#pragma unroll 1
+              for (int cc = 0; cc < HD / 16; ++cc) {
+                uint32_t o[16];
+                tmem_ld16(o_col + cc * 16, o);
+                tmem_wait_ld();
 #pragma unroll
-            for (int cc = 0; cc < HD / 32; ++cc) {
-              uint32_t o[32];
-              tmem_ld32(o_col + cc * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              tmem_st32(o_col + cc * 32, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                tmem_st16(o_col + cc * 16, o);
+              }
             }
           }
-          const uint64_t nm2 = f2_pack(-m, -m);
-          uint64_t l2 = 0;
-#pragma unroll
-          for (int j = 0; j < 128; j += 2) {
-            const uint64_t x = ffma2(f2_pack(s[j], s[j + 1]), zs2, nm2);
-            const float e0 = ex2_ftz(f2_lo(x)), e1 = ex2_ftz(f2_hi(x));
-            l2 = fadd2(l2, f2_pack(e0, e1));
-            pk[j / 2] = pack2<BF16>(e0, e1);
-          }
-          l += f2_lo(l2) + f2_hi(l2);
-        } else {
-          const uint64_t nt2 = f2_pack(-m, -m);
-#pragma unroll
-          for (int j = 0; j < 128; j += 2) {
-            const uint64_t x = ffma2(f2_pack(s[j], s[j + 1]), zs2, nt2);
-            uint64_t d = f2_pack(fmaxf(f2_lo(x), 0.f), fmaxf(f2_hi(x), 0.f));
-            if (NORM == HFAN_ENTMAX15) d = fmul2(d, d);
-            pk[j / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
-          }
         }
-      } else {
+        const uint64_t nm2 = f2_pack(-m, -m);
+        uint64_t l2 = 0;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) pk[j] = 0u;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const uint64_t x = ffma2(f2_pack(s[64 * half + j], s[64 * half + j + 1]), zs2, nm2);
+            if (NORM == HFAN_SOFTMAX1) {
+              const float e0 = ex2_ftz(f2_lo(x)), e1 = ex2_ftz(f2_hi(x));
+              l2 = fadd2(l2, f2_pack(e0, e1));
+              pk[j / 2] = pack2<BF16>(e0, e1);
+            } else {
+              uint64_t d = f2_pack(fmaxf(f2_lo(x), 0.f), fmaxf(f2_hi(x), 0.f));
+              if (NORM == HFAN_ENTMAX15) d = fmul2(d, d);
+              pk[j / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
+            }
+          }
+          tmem_st32(s_col + half * 32, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          warp_arrive(&bars->p_full[q][half]);
+        }
+        l += f2_lo(l2) + f2_hi(l2);
       }
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc) tmem_st32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(pk + cc * 32));
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(&bars->p_full[q]);
-    }
-    if (ok && nt > 0) ok = wait_warp(&bars->o_full[q], 0, abort_flag);
-    tc_fence_after();
-    if (!ok && lane == 0) fail(p, ctl);
-    const bool last = parts == 1;
-    if (NORM == HFAN_SOFTMAX1 && last) l += exp2f(-m);  // the implicit zero logit
-    const float inv = NORM == HFAN_SOFTMAX1 && last ? 1.f / l : 1.f;
-    if (warp_on || last) {
-#pragma unroll
+      // ---- the piece's result
+      if (ok) ok = wait_warp(&bars->o_full[q], mine & 1, abort_flag);
+      ++mine;
+      tc_fence_after();
+      const int row_in_unit = q * kTileRows + r;
+      if (NORM == HFAN_SOFTMAX1 && pc.whole) l += exp2f(-m);  // the implicit zero logit
+      const float inv = NORM == HFAN_SOFTMAX1 && pc.whole ? 1.f / l : 1.f;
+      T* dst = static_cast<T*>(p.o) + (int64_t)(u.g.q_start + i) * p.o_st + (int64_t)h * p.o_sh;
+      float* part = ws.o + ((int64_t)pc.slot * kUnitRows + row_in_unit) * HD;
+#pragma unroll 1
       for (int cc = 0; cc < HD / 32; ++cc) {
         uint32_t o[32];
-        if (nt > 0 && ok) {
+        if (ok) {
           tmem_ld32(o_col + cc * 32, o);
           tmem_wait_ld();
         } else {
@@ -343,8 +410,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           for (int j = 0; j < 32; ++j) o[j] = 0u;
         }
         if (!row_ok) continue;
-        if (last) {
-          T* dst = static_cast<T*>(p.o) + (int64_t)(g.q_start + i) * p.o_st + (int64_t)h * p.o_sh + cc * 32;
+        if (pc.whole) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 v;
@@ -352,23 +418,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             v.y = pack2<BF16>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
             v.z = pack2<BF16>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
             v.w = pack2<BF16>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + j) = v;
+            *reinterpret_cast<uint4*>(dst + cc * 32 + j) = v;
           }
         } else {
-          uint4* dst = reinterpret_cast<uint4*>(ws.o + ((int64_t)split * p.rows_total * p.hq + srow) * HD + cc * 32);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(part + cc * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         }
       }
-    }
-    if (row_ok) {
-      if (last && NORM == HFAN_SOFTMAX1) {
-        p.stats[si] = m;
-        p.stats[(int64_t)p.hq * p.rows_total + si] = l;
+      tc_fence_before();
+      warp_arrive(&bars->o_empty[q]);
+      if (NORM == HFAN_SOFTMAX1 && row_ok) {
+        if (pc.whole) {
+          p.stats[si] = m;
+          p.stats[(int64_t)p.hq * p.rows_total + si] = l;
+        } else {
+          ws.ml[(int64_t)pc.slot * kUnitRows + row_in_unit] = make_float2(m, l);
+        }
+        if (pc.kt0 == 0 && rg == 0)
+          ws.info[(int64_t)(u.g.q_start + i) * p.hkv + u.kvh] = make_int4(pc.u0, u.tiles, row_in_unit, src.quota);
       }
-      if (!last && NORM == HFAN_SOFTMAX1) ws.ml[(int64_t)split * p.rows_total * p.hq + srow] = make_float2(m, l);
-      if (split == 0 && ws.parts != nullptr) ws.parts[srow] = parts;
     }
+    if (!ok && lane == 0) fail(p, ctl);
   }
 
   tc_fence_before();
@@ -376,55 +447,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
-  }
-}
-
-// Joins the parts of a row: one warp per (token, head).
-template <int HD, typename T, int NORM>
-__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p, const ChunkWs ws, int splits) {
-  const int64_t rows = (int64_t)p.rows_total * p.hq, row = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const int parts = min(ws.parts[row], splits);  // (a row that no sequence owns has none)
-  if (parts < 2) return;
-  const int tok = (int)(row / p.hq), h = (int)(row - (int64_t)tok * p.hq);
-  constexpr int N = HD / 32;
-  float m = 0.f, l = 0.f;
-  if (NORM == HFAN_SOFTMAX1) {
-    for (int s = lane; s < parts; s += 32) m = fmaxf(m, ws.ml[s * rows + row].x);
-    m = warp_max(m);
-    for (int s = lane; s < parts; s += 32) {
-      const float2 x = ws.ml[s * rows + row];
-      l += x.y * exp2f(x.x - m);
-    }
-    l = warp_sum(l) + exp2f(-m);
-  }
-  float acc[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float f = NORM == HFAN_SOFTMAX1 ? exp2f(ws.ml[s * rows + row].x - m) : 1.f;
-    const float* o = ws.o + (s * rows + row) * HD + lane * N;
-    if constexpr (N == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(o);
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
-      acc[2] = fmaf(f, x.z, acc[2]);
-      acc[3] = fmaf(f, x.w, acc[3]);
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(o);
-      acc[0] = fmaf(f, x.x, acc[0]);
-      acc[1] = fmaf(f, x.y, acc[1]);
-    }
-  }
-  const float inv = NORM == HFAN_SOFTMAX1 ? 1.f / l : 1.f;
-  T* dst = static_cast<T*>(p.o) + (int64_t)tok * p.o_st + (int64_t)h * p.o_sh + lane * N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) dst[e] = from_f32<T>(acc[e] * inv);
-  if (NORM == HFAN_SOFTMAX1 && lane == 0) {
-    p.stats[(int64_t)h * p.rows_total + tok] = m;
-    p.stats[(int64_t)p.hq * p.rows_total + (int64_t)h * p.rows_total + tok] = l;
   }
 }
 
@@ -636,70 +658,30 @@ ChunkPlan plan_of(const AttnParams& p) {
   // every sequence may leave one part-filled pair
   const int64_t pairs = p.rows_total / (2 * c.tpb) + (p.batch < p.rows_total ? p.batch : p.rows_total);
   c.pairs = (int)(pairs < 1 ? 1 : pairs);
-  const int ktiles = (p.len_k + kTileKeys - 1) / kTileKeys;
-  // Sparse: this kernel serves what the scan flagged, which nobody knows yet.
-  if (p.norm != HFAN_SOFTMAX1) {
-    c.splits = 1;
-    c.span = ktiles > 0 ? ktiles : 1;
-    return c;
-  }
-  // One wave of CTAs over the SMs; a part shorter than four key tiles would
-  // pay more for its prologue and its partial result than it saves.
-  const int64_t units = (int64_t)c.pairs * p.hkv;
-  int64_t splits = units > 0 ? sm_count() / units : 1;
-  if (splits > (ktiles + 3) / 4) splits = (ktiles + 3) / 4;
-  if (splits < 1) splits = 1;
-  c.span = (int)((ktiles + splits - 1) / splits);
-  if (c.span < 1) c.span = 1;
-  c.splits = (ktiles + c.span - 1) / c.span;
-  if (c.splits < 1) c.splits = 1;
   return c;
-}
-
-struct WsLayout {
-  int64_t o, ml, parts, flags, total;
-};
-WsLayout ws_layout(const AttnParams& p, const ChunkPlan& c) {
-  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
-  const int64_t rows = (int64_t)p.rows_total * p.hq;
-  WsLayout w{0, 0, 0, 0, 0};
-  if (p.norm != HFAN_SOFTMAX1) w.total = up((int64_t)c.pairs * p.hkv * 4);
-  if (c.splits < 2) return w;
-  w.ml = up(rows * c.splits * p.d * 4);
-  w.parts = w.ml + up(rows * c.splits * 8);
-  w.total = w.parts + up(rows * 4);
-  return w;
 }
 
 template <int HD, bool BF16, int NORM>
 cudaError_t fwd_t(const AttnParams& p, const ChunkPlan& c, void* workspace, cudaStream_t s) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   CUtensorMap tq, tk, tv;
   if (!make_row_map(&tq, p, BF16, c) || !make_page_map(&tk, p.k, p.k_st, p.k_sh, p, BF16, c) ||
       !make_page_map(&tv, p.v, p.v_st, p.v_sh, p, BF16, c))
     return cudaErrorInvalidValue;
-  const WsLayout w = ws_layout(p, c);
-  ChunkWs ws{nullptr, nullptr, nullptr, nullptr};
-  if (c.splits > 1) {
-    uint8_t* base = static_cast<uint8_t*>(workspace);
-    ws.o = reinterpret_cast<float*>(base + w.o);
-    ws.ml = reinterpret_cast<float2*>(base + w.ml);
-    ws.parts = reinterpret_cast<int*>(base + w.parts);
-  }
-  if (NORM != HFAN_SOFTMAX1) {
-    ws.flags = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + w.flags);
-    const cudaError_t e = chunk_sparse_scan(BF16 ? HFAN_BFLOAT16 : HFAN_FLOAT16, p, c, ws.flags, s);
-    if (e != cudaSuccess) return e;
-  }
-  auto kernel = chunk_fwd_kernel<HD, BF16, NORM>;
   constexpr int smem = ChunkLayout<HD>::TOTAL;
   cudaError_t e = allow_smem<chunk_fwd_kernel<HD, BF16, NORM>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(c.pairs, p.hkv, c.splits), kChunkThreads, smem, s>>>(tq, tk, tv, p, c, ws);
-  if (c.splits > 1) {
-    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    const int64_t rows = (int64_t)p.rows_total * p.hq;
-    combine_kernel<HD, T, NORM><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(p, ws, c.splits);
+  if (NORM == HFAN_SOFTMAX1) {
+    const int ctas = sm_count();
+    const PieceWs ws = piece_ws(p, ctas, kUnitRows, workspace);
+    chunk_fwd_kernel<HD, BF16, NORM><<<ctas, kChunkThreads, smem, s>>>(tq, tk, tv, p, c, ws, nullptr);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    return launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, s, p, ws, c.group);
   }
+  int* flags = static_cast<int*>(workspace);
+  e = chunk_sparse_scan(BF16 ? HFAN_BFLOAT16 : HFAN_FLOAT16, p, c, flags, s);
+  if (e != cudaSuccess) return e;
+  chunk_fwd_kernel<HD, BF16, NORM><<<dim3(c.pairs, p.hkv), kChunkThreads, smem, s>>>(tq, tk, tv, p, c, PieceWs{}, flags);
   return cudaGetLastError();
 }
 
@@ -737,6 +719,9 @@ bool keys_supported(int dtype, const AttnParams& p) {
   // a swizzle atom is 8 rows of a page; masked scores are -inf before the scaling
   if (p.page_size % 8 != 0 || !(p.scale > 0.f) || p.hq / p.hkv > kTileRows) return false;
   if (p.num_cache_tokens < 1 || p.num_cache_tokens > 0x7fffffffll) return false;
+  // key tiles of the whole batch are counted in 32 bits
+  const ChunkPlan c = plan_of(p);
+  if ((int64_t)c.pairs * p.hkv * (p.len_k / kTileKeys + 1) > 0x3fffffff) return false;
   return aligned16(p.q) && aligned16(p.k) && stride_ok(p.q_st) && stride_ok(p.q_sh) && stride_ok(p.k_st) &&
          stride_ok(p.k_sh);
 }
@@ -750,7 +735,8 @@ bool chunk_tc_supported(int dtype, const AttnParams& p) {
 
 int64_t chunk_tc_workspace(const AttnParams& p, bool weights) {
   const ChunkPlan c = plan_of(p);
-  return chunk_few_applies(p, c, weights) ? chunk_few_workspace(p, c, weights) : ws_layout(p, c).total;
+  if (p.norm != HFAN_SOFTMAX1) return (int64_t)c.pairs * p.hkv * 4;  // flags
+  return chunk_few_applies(p, c, weights) ? chunk_few_workspace(p, c, weights) : piece_layout(p, sm_count(), kUnitRows).total;
 }
 
 static cudaError_t dense_fwd(int dtype, const AttnParams& p, const ChunkPlan& c, void* workspace, cudaStream_t s) {

@@ -36,16 +36,19 @@ using namespace tc;
 constexpr int kFewThreads = 192;
 constexpr float kRescale = 8.f;
 
+constexpr int kSumStride = 132;  // floats; rows of 128 start in different banks
+
 template <int HD, int NC>
 struct FewLayout {
-  static constexpr int NH = HD / 64, NS = HD == 128 ? 6 : 10;
+  static constexpr int NH = HD / 64, NS = HD == 128 ? (NC == 16 ? 6 : 5) : 10;
   static constexpr uint32_t TILE = NH * kHalf;
   static constexpr uint32_t QB = NH * NC * 128;  // one Q buffer
   static constexpr uint32_t PB = 2 * NC * 128;   // one P^T buffer
   static constexpr uint32_t Q = NS * TILE;       // two buffers: the next piece's Q comes early
   static constexpr uint32_t P = Q + 2 * QB;
   static constexpr uint32_t RED = P + 2 * PB;    // float [4][NC]
-  static constexpr uint32_t BARS = RED + 4 * NC * 4;
+  static constexpr uint32_t SUMS = RED + 4 * NC * 4;  // float [NC][kSumStride]
+  static constexpr uint32_t BARS = SUMS + NC * kSumStride * 4;
   // (at HD = 64 an MMA's second 64-wide block lies one half tile further on, past the last stage's end)
   static constexpr uint32_t TOTAL = BARS + 512 + 1024 + (HD == 64 ? kHalf : 0);
 };
@@ -56,6 +59,10 @@ struct FewBars {
   int abort, never;
 };
 static_assert(sizeof(FewBars) <= 512, "FewBars outgrew its place");
+
+static_assert(FewLayout<128, 16>::TOTAL <= 232448 && FewLayout<128, 32>::TOTAL <= 232448 &&
+                  FewLayout<64, 16>::TOTAL <= 232448 && FewLayout<64, 32>::TOTAL <= 232448,
+              "more shared memory than a block can have");
 
 // Scores kept of a key: its packed rows, rounded up to whole vectors.
 __host__ __device__ __forceinline__ int score_floats(const ChunkPlan& c) { return (c.tpb * c.group + 3) & ~3; }
@@ -81,6 +88,12 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   FewBars* bars = reinterpret_cast<FewBars*>(smem + L::BARS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  allow_dependents();
+  if (warp == 4 && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&bars->full[s], 1);
@@ -110,11 +123,6 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 
   if (warp == 4) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      prefetch_tmap(&tm_q);
-      prefetch_tmap(&tm_k);
-      prefetch_tmap(&tm_v);
-    }
     bool ok = true;
     int issued = 0, pieces = 0;
     while (ok && walk.next()) {
@@ -209,6 +217,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const float zs = p.scale * kLog2e;
     float* red = reinterpret_cast<float*>(smem + L::RED);
+    float* sums = reinterpret_cast<float*>(smem + L::SUMS);
     const uint32_t p_base = smem_u32(smem + L::P);
     // this key's 16-byte chunk of a P^T row, before the row's swizzle
     const uint32_t p_half = (uint32_t)(r >> 6) * NC * 128, p_chunk = (uint32_t)((r >> 3) & 7), p_in = (uint32_t)(r & 7) * 2;
@@ -254,8 +263,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           // some row passed its reference: the tile's row maxima over the four warps
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
-            const float w = warp_max(x[e]);
-            if (lane == 0) red[warp * NC + e] = w;
+            // only maxima above m + 2^3 > 0 matter, and positive floats compare as integers
+            const int w = __reduce_max_sync(0xffffffffu, __float_as_int(fmaxf(x[e], 0.f)));
+            if (lane == 0) red[warp * NC + e] = __int_as_float(w);
           }
           named_bar_sync(1, 128);
           float alpha[NC];
@@ -316,35 +326,51 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       tmem_wait_ld();
       tc_fence_before();
       warp_arrive(&bars->o_empty);
+      // sums of l over the keys' threads: eight lanes add up a row's 128 values
 #pragma unroll
-      for (int e = 0; e < NC; ++e) {
-        const float w = warp_sum(l[e]);
-        if (lane == 0) red[warp * NC + e] = w;
+      for (int e = 0; e < NC; ++e) sums[e * kSumStride + r] = l[e];
+      named_bar_sync(1, 128);
+#pragma unroll
+      for (int e0 = 0; e0 < NC; e0 += 16) {
+        const float4* s4 = reinterpret_cast<const float4*>(sums + (e0 + (r >> 3)) * kSumStride + (r & 7) * 16);
+        float w = 0.f;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float4 v = s4[y];
+          w += (v.x + v.y) + (v.z + v.w);
+        }
+#pragma unroll
+        for (int y = 4; y > 0; y >>= 1) w += __shfl_xor_sync(0xffffffffu, w, y);
+        if ((r & 7) == 0) red[e0 + (r >> 3)] = w;
       }
       named_bar_sync(1, 128);
-      const int64_t tok_g = u.g.q_start + u.tok0;
+      int64_t tok = u.g.q_start + u.tok0;
+      int h = u.kvh * c.group;
 #pragma unroll
       for (int e = 0; e < NC; ++e) {
-        if (e >= rows) continue;
-        float sum = red[e] + red[NC + e] + red[2 * NC + e] + red[3 * NC + e];
-        const int64_t tok = tok_g + e / c.group;
-        const int h = u.kvh * c.group + e % c.group;
-        if (pc.whole) {
-          sum += exp2f(-m[e]);  // the implicit zero logit
-          if (r < HD)
-            static_cast<T*>(p.o)[tok * p.o_st + (int64_t)h * p.o_sh + r] = from_f32<T>(__uint_as_float(o[e]) * (1.f / sum));
-          if (r == 0) {
-            p.stats[(int64_t)h * p.rows_total + tok] = m[e];
-            p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = sum;
+        if (e < rows) {
+          float sum = red[e];
+          if (pc.whole) {
+            sum += exp2f(-m[e]);  // the implicit zero logit
+            if (r < HD)
+              static_cast<T*>(p.o)[tok * p.o_st + (int64_t)h * p.o_sh + r] = from_f32<T>(__uint_as_float(o[e]) * (1.f / sum));
+            if (r == 0) {
+              p.stats[(int64_t)h * p.rows_total + tok] = m[e];
+              p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = sum;
+            }
+          } else {
+            const int64_t at = (int64_t)pc.slot * ws.rows + e;
+            if (r < HD) ws.o[at * HD + r] = __uint_as_float(o[e]);
+            if (r == 0) ws.ml[at] = make_float2(m[e], sum);
           }
-        } else {
-          const int64_t at = (int64_t)pc.slot * ws.rows + e;
-          if (r < HD) ws.o[at * HD + r] = __uint_as_float(o[e]);
-          if (r == 0) ws.ml[at] = make_float2(m[e], sum);
+          if (++h == (u.kvh + 1) * c.group) {
+            h = u.kvh * c.group;
+            ++tok;
+          }
         }
       }
       if (pc.kt0 == 0 && r < u.ntok)
-        ws.info[(tok_g + r) * p.hkv + u.kvh] = make_int4(pc.u0, u.tiles, r * c.group, walk.quota);
+        ws.info[(int64_t)(u.g.q_start + u.tok0 + r) * p.hkv + u.kvh] = make_int4(pc.u0, u.tiles, r * c.group, walk.quota);
       named_bar_sync(1, 128);  // red may be written again
       ++pieces;
     }
@@ -362,7 +388,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 template <int NC>
 __global__ void __launch_bounds__(256) few_weights_kernel(const AttnParams p, const ChunkPlan c, const float* scores,
                                                           float* kw, int64_t ldw) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_predecessor();
   __shared__ float consts[NC];
   const int b = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
   const Geometry g = geometry(p, b);
@@ -416,7 +442,7 @@ cudaError_t run(const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw,
   if (e != cudaSuccess) return e;
   few_kernel<HD, BF16, NC><<<ctas, kFewThreads, smem, s>>>(tq, tk, tv, p, c, ws, scores);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  e = launch_dependent(combine_pieces_kernel<HD, T, HFAN_SOFTMAX1>, dim3(p.rows_total * p.hkv), 128, s, p, ws, c.group);
+  e = launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, s, p, ws, c.group);
   if (e != cudaSuccess || kw == nullptr) return e;
   return launch_dependent(few_weights_kernel<NC>, dim3((p.len_k + 255) / 256, p.hkv, p.batch), 256, s, p, c,
                           static_cast<const float*>(scores), kw, ldw);

@@ -5,14 +5,15 @@
 // form one line that is cut into equal stretches, one per CTA: every SM gets
 // the same number of tiles however ragged the lengths are.  A stretch may start
 // and end inside a unit, so a CTA has at most two partial results, its first
-// piece and its last; combine_kernel joins the pieces of a unit.
+// piece and its last; combine_pieces_kernel joins the pieces of a unit.
 #pragma once
 
 #include "paged_chunk.cuh"
+#include "tc_ptx.cuh"
 
 namespace hfan {
 
-// What the pieces of a unit leave for combine_kernel.
+// What the pieces of a unit leave for combine_pieces_kernel.
 struct PieceWs {
   float* o;    // [2 * ctas][rows of a unit][D] unscaled O of a partial piece
   float2* ml;  // [2 * ctas][rows of a unit] (reference m, sum l)
@@ -43,16 +44,19 @@ class Walk {
   // Whole-warp call: finds the start of this CTA's stretch.
   __device__ __forceinline__ Walk(const AttnParams& p, int per) : p_(p), per_(per) {
     const int lane = threadIdx.x & 31;
-    int total = 0;
-    for (int base = 0; base < p.batch; base += 32)
-      total += __reduce_add_sync(0xffffffffu, base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0);
+    int total = 0, w0 = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int w = base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0;
+      if (base == 0) w0 = w;
+      total += __reduce_add_sync(0xffffffffu, w);
+    }
     quota = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 2);
     at_ = (int)blockIdx.x * quota;
     end_ = min(at_ + quota, total);
     if (at_ >= end_) return;
     int before = 0;
     for (int base = 0;; base += 32) {
-      const int w = base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0;
+      const int w = base == 0 ? w0 : (base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0);
       int inc = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -137,9 +141,10 @@ class Walk {
 };
 
 // Joins the pieces of split units: one block per (token, KV head) and its G rows.
-template <int HD, typename T, int NORM>
+template <int HD, typename T>
 __global__ void __launch_bounds__(128) combine_pieces_kernel(const AttnParams p, const PieceWs ws, int group) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the pieces are still being computed
+  tc::allow_dependents();
+  tc::wait_for_predecessor();  // (set up while the pieces are still being computed)
   const int tok = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
   const int4 f = ws.info[blockIdx.x];
   // (a token that no sequence owns has no info: kept inside the workspace)
@@ -147,37 +152,40 @@ __global__ void __launch_bounds__(128) combine_pieces_kernel(const AttnParams p,
   const int last = min(max((f.x + f.y - 1) / quota, first), ws.ctas - 1);
   if (last == first) return;
   const int head = 2 * first + (f.x == first * quota ? 0 : 1);  // slot of the unit's first piece; the others lead their CTA
-  constexpr int LPR = HD / 4;                                   // lanes of a row
+  constexpr int LPR = HD / 4;  // lanes of a row: they also share the row's (m, l) loads
+  const int parts = last - first + 1, lane = threadIdx.x % LPR, d = lane * 4;
+  const unsigned mask = LPR == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
   for (int g = threadIdx.x / LPR; g < group; g += 128 / LPR) {
-    const int d = (threadIdx.x % LPR) * 4, row = min(max(f.z, 0), ws.rows - group) + g;
+    const int row = min(max(f.z, 0), ws.rows - group) + g;
+    auto at = [&](int j) { return (int64_t)(j == 0 ? head : 2 * (first + j)) * ws.rows + row; };
     float m = 0.f, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (NORM == HFAN_SOFTMAX1)
-      for (int c = first; c <= last; ++c) m = fmaxf(m, ws.ml[(int64_t)(c == first ? head : 2 * c) * ws.rows + row].x);
-#pragma unroll 4
-    for (int c = first; c <= last; ++c) {
-      const int64_t at = (int64_t)(c == first ? head : 2 * c) * ws.rows + row;
-      const float4 x = *reinterpret_cast<const float4*>(ws.o + at * HD + d);
-      float s = 1.f;
-      if (NORM == HFAN_SOFTMAX1) {
-        const float2 ml = ws.ml[at];
-        s = exp2f(ml.x - m);
-        l += ml.y * s;
+    for (int j = lane; j < parts; j += LPR) m = fmaxf(m, ws.ml[at(j)].x);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o, LPR));
+    for (int j0 = 0; j0 < parts; j0 += LPR) {
+      const float2 ml = j0 + lane < parts ? ws.ml[at(j0 + lane)] : make_float2(kNegInf, 0.f);
+      const float sj = exp2f(ml.x - m);
+      l += ml.y * sj;
+      const int n = min(LPR, parts - j0);
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(ws.o + at(j0 + j) * HD + d);
+        const float s = __shfl_sync(mask, sj, j, LPR);
+        acc.x = fmaf(s, x.x, acc.x);
+        acc.y = fmaf(s, x.y, acc.y);
+        acc.z = fmaf(s, x.z, acc.z);
+        acc.w = fmaf(s, x.w, acc.w);
       }
-      acc.x = fmaf(s, x.x, acc.x);
-      acc.y = fmaf(s, x.y, acc.y);
-      acc.z = fmaf(s, x.z, acc.z);
-      acc.w = fmaf(s, x.w, acc.w);
     }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) l += __shfl_xor_sync(mask, l, o, LPR);
+    l += exp2f(-m);  // the implicit zero logit
+    const float inv = 1.f / l;
     const int h = kvh * group + g;
-    float inv = 1.f;
-    if (NORM == HFAN_SOFTMAX1) {
-      l += exp2f(-m);  // the implicit zero logit
-      inv = 1.f / l;
-      if (d == 0) {
-        p.stats[(int64_t)h * p.rows_total + tok] = m;
-        p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = l;
-      }
+    if (d == 0) {
+      p.stats[(int64_t)h * p.rows_total + tok] = m;
+      p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = l;
     }
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     uint2 y;

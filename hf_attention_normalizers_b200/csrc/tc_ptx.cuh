@@ -92,6 +92,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// ---------------------------------------------------------------- dependent launches
+// Lets the next kernel of the stream (launched as a dependent) be set up while
+// this one runs; it waits in wait_for_predecessor before it reads anything.
+__device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- shared memory
 // Explicit shared-space accesses: through a generic pointer a scattered store
 // costs a warp about 45 cycles of issue, these a few.
