@@ -12,15 +12,16 @@
 //                   sum need no exchange, and writes P over S as packed
 //                   16-bit pairs (the A operand of P V).
 //   warp 8          producer: Q of a piece, then K0 V0 K1 V1 ... through one ring.
-//   warps 9, 10     MMA issuers of tile 0 / 1: S = Q K^T, then O += P V, then
-//                   the next S over the P just consumed.
+//   warps 9, 10     MMA issuers of tile 0 / 1.
 //
-// The two tiles are independent chains that share the K and V stages: while
-// one chain's row warps exponentiate, the tensor pipe works for the other.
+// The two tiles are independent chains that share the K and V stages.  A chain
+// works in halves of a key tile (64 keys) with two S buffers: while the row
+// warps exponentiate half j, the tensor pipe has S of j + 1 ready and works on
+// O += P V of j - 1 and S of j + 1 into the buffer that P of j - 1 leaves, so
+// neither side waits for the other's latency.  (One 128-key S buffer a chain,
+// all that fits beside O, left the row warps waiting 1700 of 4600 cycles.)
 // softmax1 keeps a reference m >= 0 (the implicit zero logit) that follows the
-// row maximum lazily: O is rescaled only when the maximum grew by more than
-// 2^8.  P V of tile t is done before S of tile t + 1 (same issuer), so the row
-// warps that hold S of t + 1 may rescale O without another wait.
+// row maximum lazily: O is rescaled only when the maximum grew by more than 2^8.
 //
 // sparsemax / entmax15 come here with their thresholds known, for the units
 // that the scan (paged_chunk_sparse.cu) could not serve from its buffers.
@@ -39,21 +40,18 @@ namespace {
 
 using namespace tc;
 
-constexpr int kChunkThreads = 384;
-// Registers of a thread: 384 x 168 at launch; the helper warpgroup (producer,
-// issuers) gives up what lets a row thread hold its S row without spills.
-constexpr int kRowRegs = 224, kHelperRegs = 56;
-static_assert(256 * kRowRegs + 128 * kHelperRegs <= 384 * 168, "more registers than the block was launched with");
+constexpr int kChunkThreads = 352;
 constexpr int kMaxRing = 8;
 constexpr float kRescale = 8.f;
 constexpr int kUnitRows = 2 * kTileRows;
+constexpr int kHalfKeys = kTileKeys / 2;
 
 template <int HD>
 constexpr int chunk_ring() { return HD == 128 ? 5 : 8; }
 
 struct ChunkBars {
   uint64_t q_full, q_empty, full[kMaxRing], empty[kMaxRing];
-  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2], drain[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_empty[2], drain[2];
 };
 struct ChunkCtl {
   uint32_t tmem;
@@ -120,7 +118,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   using Source = typename std::conditional<NORM == HFAN_SOFTMAX1, Stretch, FlaggedUnit>::type;
   constexpr int NH = L::NH, NS = L::NS;
-  constexpr uint32_t IDESC_QK = idesc_f16(BF16, 128, 128, false, false);
+  constexpr uint32_t IDESC_QK = idesc_f16(BF16, 128, kHalfKeys, false, false);
   constexpr uint32_t IDESC_PV = idesc_f16(BF16, 128, HD, false, true);
 
   extern __shared__ uint8_t smem_raw[];
@@ -143,10 +141,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&bars->empty[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_full[s][0], 4);
-      mbar_init(&bars->p_full[s][1], 4);
-      mbar_init(&bars->o_full[s], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars->s_full[s][h], 1);
+        mbar_init(&bars->p_full[s][h], 4);
+      }
+      mbar_init(&bars->pv_done[s], 1);
       mbar_init(&bars->o_empty[s], 4);
       mbar_init(&bars->drain[s], 1);
     }
@@ -159,11 +158,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;  // S0 | S1 | O0 | O1, 128 columns each
+  const uint32_t tmem = ctl->tmem;  // S of tile 0 (two halves) | of tile 1 | O0 | O1, 128 columns each
   volatile int* abort_flag = &ctl->abort;
 
   if (warp >= 8) {
-    set_max_regs<kHelperRegs, false>();
     if (warp == 8) {
       // ---------------------------------------------------------- producer
       bool ok = true;
@@ -203,67 +201,63 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&bars->full[i % NS], (i / NS) & 1, &ctl->never);
       }
       __syncwarp();
-    } else if (warp < 11) {  // (warp 11 fills the warpgroup)
+    } else {
       // ---------------------------------------------------------- MMA issuers
       const int q = warp - 9;
       const uint32_t q_base = smem_u32(smem + q * L::TILE), ring = smem_u32(smem + L::RING);
       const uint32_t s_col = tmem + q * 128, o_col = tmem + 256 + q * 128;
       bool ok = true;
-      int st = 0, ph = 0, it = 0, pieces = 0, mine = 0;  // mine: pieces in which this tile has rows
-      auto step = [&]() {
-        if (++st == NS) {
-          st = 0;
-          ph ^= 1;
-        }
-      };
+      int items = 0, pieces = 0, mine = 0;  // ring items and pieces so far; pieces in which this tile has rows
+      int jj = 0;                           // halves of those pieces
       while (src.next()) {
+        const int nt = src.piece.nt;
         if (lane == 0 && ok) {
-          const int nt = src.piece.nt;
           ok = mbar_wait(&bars->q_full, pieces & 1, abort_flag);
           if (q == 1 && src.u.ntok <= c.tpb) {
             // no rows: the stages are only passed on
-            for (int t = 0; t < 2 * nt && ok; ++t) {
-              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
-              mbar_arrive(&bars->empty[st]);
-              step();
+            for (int x = items; x < items + 2 * nt && ok; ++x) {
+              if (!(ok = mbar_wait(&bars->full[x % NS], (x / NS) & 1, abort_flag))) break;
+              mbar_arrive(&bars->empty[x % NS]);
             }
             mbar_arrive(&bars->q_empty);
           } else {
-            for (int t = 0; t < nt && ok; ++t, ++it) {
-              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
+            // S of half j into buffer j & 1, which P V of half j - 2 has left
+            auto issue_s = [&](int j) -> bool {
+              const int item = items + 2 * (j >> 1), st = item % NS, h = j & 1;
+              if (h == 0 && !mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag)) return false;
               tc_fence_after();
 #pragma unroll
               for (int kk = 0; kk < HD / 16; ++kk) {
                 const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-                mma_f16_ss(s_col, sw128_desc(q_base + o, 16, 1024), sw128_desc(ring + st * L::TILE + o, 16, 1024), IDESC_QK,
-                           kk > 0);
+                mma_f16_ss(s_col + h * kHalfKeys, sw128_desc(q_base + o, 16, 1024),
+                           sw128_desc(ring + st * L::TILE + o + h * kHalfKeys * 128, 16, 1024), IDESC_QK, kk > 0);
               }
-              mma_commit(&bars->s_full[q]);
-              mma_commit(&bars->empty[st]);
-              if (t + 1 == nt) mma_commit(&bars->q_empty);
-              step();
-              if (!(ok = mbar_wait(&bars->full[st], ph, abort_flag))) break;
-              // P comes in halves: its first 64 keys are multiplied while the
-              // row warps exponentiate the others
-              if (t == 0 && !(ok = mbar_wait(&bars->o_empty[q], (mine & 1) ^ 1, abort_flag))) break;
+              mma_commit(&bars->s_full[q][h]);
+              if (h == 1) mma_commit(&bars->empty[st]);
+              if (j == 2 * nt - 1) mma_commit(&bars->q_empty);
+              return true;
+            };
+            ok = ok && issue_s(0) && issue_s(1);
+            for (int j = 0; j < 2 * nt && ok; ++j, ++jj) {
+              const int item = items + 2 * (j >> 1) + 1, st = item % NS, h = j & 1;
+              if (h == 0 && !(ok = mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag))) break;
+              if (j == 0 && !(ok = mbar_wait(&bars->o_empty[q], (mine & 1) ^ 1, abort_flag))) break;
+              if (!(ok = mbar_wait(&bars->p_full[q][h], (jj >> 1) & 1, abort_flag))) break;
+              tc_fence_after();
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!(ok = mbar_wait(&bars->p_full[q][half], it & 1, abort_flag))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  mma_f16_ts(o_col, s_col + kk * 8, sw128_desc(ring + st * L::TILE + kk * 16 * 128, kHalf, 1024), IDESC_PV,
-                             t > 0 || kk > 0);
-              }
-              if (!ok) break;
-              mma_commit(&bars->empty[st]);
-              if (t + 1 == nt) mma_commit(&bars->o_full[q]);
-              step();
+              for (int kk = 0; kk < kHalfKeys / 16; ++kk)
+                mma_f16_ts(o_col, s_col + h * kHalfKeys + kk * 8,
+                           sw128_desc(ring + st * L::TILE + (h * kHalfKeys + kk * 16) * 128, kHalf, 1024), IDESC_PV,
+                           j > 0 || kk > 0);
+              mma_commit(&bars->pv_done[q]);
+              if (h == 1) mma_commit(&bars->empty[st]);
+              if (j + 2 < 2 * nt) ok = issue_s(j + 2);
             }
             ++mine;
           }
-          ++pieces;
         }
+        items += 2 * nt;
+        ++pieces;
         __syncwarp();
       }
       if (lane == 0 && !ok) {
@@ -275,14 +269,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ row warps
-    set_max_regs<kRowRegs, true>();
     const int q = warp >> 2, r = threadIdx.x & 127;
     const int rt = r / c.group, rg = r - rt * c.group;  // token of the tile, head of the group
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_addr + q * 128, o_col = tmem + lane_addr + 256 + q * 128;
     const float zs = NORM == HFAN_SOFTMAX1 ? p.scale * kLog2e : (NORM == HFAN_SPARSEMAX ? p.scale : 0.5f * p.scale);
     bool ok = true;
-    int it = 0, mine = 0;
+    int jj = 0;     // halves so far
     int items = 0;  // ring items of the pieces before this one
     while (src.next()) {
       const Unit& u = src.u;
@@ -300,15 +293,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int64_t si = row_ok ? stat_index(p, u.g, h, i) : 0;
       float m = 0.f, l = 0.f;
       if (NORM != HFAN_SOFTMAX1) m = row_ok ? p.stats[si] : kPosInf;  // the threshold
-      for (int t = 0; t < pc.nt; ++t, ++it) {
-        if (ok) ok = wait_warp(&bars->s_full[q], it & 1, abort_flag);
+      for (int j = 0; j < 2 * pc.nt; ++j, ++jj) {
+        const int h2 = j & 1, kb = pc.kt0 * kTileKeys + j * kHalfKeys;
+        const uint32_t s_half = s_col + h2 * kHalfKeys;
+        if (ok) ok = wait_warp(&bars->s_full[q][h2], (jj >> 1) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const int kb = (pc.kt0 + t) * kTileKeys;
-        if (kb + kTileKeys > u.g.k_len) {
+        if (h2 == 0 && kb + kTileKeys > u.g.k_len) {
           // V rows past the sequence hold stale or foreign values: zeroed, since
           // 0 x NaN would reach O (both tiles' warps write the same zeros)
-          const int item = v0 + 2 * t, vst = item % NS, lo = max(u.g.k_len - kb, 0);
+          const int item = v0 + j, vst = item % NS, lo = max(u.g.k_len - kb, 0);
           if (!(ok = wait_warp(&bars->full[vst], (item / NS) & 1, abort_flag))) break;
           uint8_t* v = smem + L::RING + vst * L::TILE;
           for (int x = r; x < (kTileKeys - lo) * 8 * NH; x += 128) {
@@ -317,82 +311,75 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           fence_proxy_async_smem();
         }
-        if (!warp_on) {
-          const uint32_t zero[32] = {};
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            tmem_st32(s_col + half * 32, zero);
-            tmem_wait_st();
-            tc_fence_before();
-            warp_arrive(&bars->p_full[q][half]);
-          }
-          continue;
-        }
-        float s[128];
-        {
-          uint32_t x[4][32];
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc) tmem_ld32(s_col + cc * 32, x[cc]);
+        uint32_t pk[32];
+        if (warp_on) {
+          uint32_t x[2][32];
+          tmem_ld32(s_half, x[0]);
+          tmem_ld32(s_half + 32, x[1]);
           tmem_wait_ld();
+          float s[64];
 #pragma unroll
-          for (int j = 0; j < 128; ++j) s[j] = __uint_as_float(x[j >> 5][j & 31]);
-        }
-        const int lim = vis - kb;
-        if (!__all_sync(0xffffffffu, lim >= kTileKeys)) {
+          for (int e = 0; e < 64; ++e) s[e] = __uint_as_float(x[e >> 5][e & 31]);
+          const int lim = vis - kb;
+          if (!__all_sync(0xffffffffu, lim >= kHalfKeys)) {
 #pragma unroll
-          for (int j = 0; j < 128; ++j) s[j] = j < lim ? s[j] : kNegInf;
-        }
-        const uint64_t zs2 = f2_pack(zs, zs);
-        if (NORM == HFAN_SOFTMAX1) {
-          const float top = max_n<128>(s) * zs;
-          if (__any_sync(0xffffffffu, top > m + kRescale)) {
-            float alpha = 1.f;
-            if (top > m + kRescale) {
-              alpha = exp2f(m - top);
-              m = top;
-              l *= alpha;
-            }
-            if (t > 0) {
+            for (int e = 0; e < 64; ++e) s[e] = e < lim ? s[e] : kNegInf;
+          }
+          if (NORM == HFAN_SOFTMAX1) {
+            const float top = max_n<64>(s) * zs;
+            if (__any_sync(0xffffffffu, top > m + kRescale)) {
+              float alpha = 1.f;
+              if (top > m + kRescale) {
+                alpha = exp2f(m - top);
+                m = top;
+                l *= alpha;
+              }
+              if (j > 0) {
+                // O holds every earlier half once P V of the last one is done
+                // (S of this one implies P V of the one before that)
+                if (!(ok = wait_warp(&bars->pv_done[q], (jj - 1) & 1, abort_flag))) break;
+                tc_fence_after();
 #pragma unroll 1
-              for (int cc = 0; cc < HD / 16; ++cc) {
-                uint32_t o[16];
-                tmem_ld16(o_col + cc * 16, o);
-                tmem_wait_ld();
+                for (int cc = 0; cc < HD / 16; ++cc) {
+                  uint32_t o[16];
+                  tmem_ld16(o_col + cc * 16, o);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                tmem_st16(o_col + cc * 16, o);
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                  tmem_st16(o_col + cc * 16, o);
+                }
               }
             }
           }
-        }
-        const uint64_t nm2 = f2_pack(-m, -m);
-        uint64_t l2 = 0;
+          const uint64_t zs2 = f2_pack(zs, zs), nm2 = f2_pack(-m, -m);
+          uint64_t l2 = 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            const uint64_t x = ffma2(f2_pack(s[64 * half + j], s[64 * half + j + 1]), zs2, nm2);
+          for (int e = 0; e < 64; e += 2) {
+            const uint64_t y = ffma2(f2_pack(s[e], s[e + 1]), zs2, nm2);
             if (NORM == HFAN_SOFTMAX1) {
-              const float e0 = ex2_ftz(f2_lo(x)), e1 = ex2_ftz(f2_hi(x));
+              const float e0 = ex2_ftz(f2_lo(y)), e1 = ex2_ftz(f2_hi(y));
               l2 = fadd2(l2, f2_pack(e0, e1));
-              pk[j / 2] = pack2<BF16>(e0, e1);
+              pk[e / 2] = pack2<BF16>(e0, e1);
             } else {
-              uint64_t d = f2_pack(fmaxf(f2_lo(x), 0.f), fmaxf(f2_hi(x), 0.f));
+              uint64_t d = f2_pack(fmaxf(f2_lo(y), 0.f), fmaxf(f2_hi(y), 0.f));
               if (NORM == HFAN_ENTMAX15) d = fmul2(d, d);
-              pk[j / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
+              pk[e / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
             }
           }
-          tmem_st32(s_col + half * 32, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          warp_arrive(&bars->p_full[q][half]);
+          l += f2_lo(l2) + f2_hi(l2);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) pk[e] = 0u;
         }
-        l += f2_lo(l2) + f2_hi(l2);
+        tmem_st32(s_half, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&bars->p_full[q][h2]);
       }
       // ---- the piece's result
-      if (ok) ok = wait_warp(&bars->o_full[q], mine & 1, abort_flag);
-      ++mine;
+      // (S of the last half implies P V of the third last: the phases of a
+      // barrier are told apart by parity, so the last two are waited for in turn)
+      if (ok) ok = wait_warp(&bars->pv_done[q], (jj - 2) & 1, abort_flag) && wait_warp(&bars->pv_done[q], (jj - 1) & 1, abort_flag);
       tc_fence_after();
       const int row_in_unit = q * kTileRows + r;
       if (NORM == HFAN_SOFTMAX1 && pc.whole) l += exp2f(-m);  // the implicit zero logit

@@ -362,16 +362,6 @@ __device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool v) {
   return r != 0;
 }
 
-// Moves registers between the warpgroups of a block: every warp of a warpgroup
-// calls it with the same count (a multiple of 8).
-template <int N, bool INC>
-__device__ __forceinline__ void set_max_regs() {
-  if constexpr (INC)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-  else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // Named barrier among `nthreads` threads (id != 0).
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
