@@ -203,54 +203,62 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       __syncwarp();
     } else {
       // ---------------------------------------------------------- MMA issuers
+      // (the whole warp walks the loops and one elected lane issues: a branch
+      // for lane 0 around them made every MMA dearer to issue, 538 against 508 us)
       const int q = warp - 9;
       const uint32_t q_base = smem_u32(smem + q * L::TILE), ring = smem_u32(smem + L::RING);
       const uint32_t s_col = tmem + q * 128, o_col = tmem + 256 + q * 128;
+      const uint64_t q_desc = sw128_desc(q_base, 16, 1024);
       bool ok = true;
       int items = 0, pieces = 0, mine = 0;  // ring items and pieces so far; pieces in which this tile has rows
       int jj = 0;                           // halves of those pieces
       while (src.next()) {
         const int nt = src.piece.nt;
-        if (lane == 0 && ok) {
-          ok = mbar_wait(&bars->q_full, pieces & 1, abort_flag);
+        if (ok) {
+          ok = wait_warp(&bars->q_full, pieces & 1, abort_flag);
           if (q == 1 && src.u.ntok <= c.tpb) {
             // no rows: the stages are only passed on
             for (int x = items; x < items + 2 * nt && ok; ++x) {
-              if (!(ok = mbar_wait(&bars->full[x % NS], (x / NS) & 1, abort_flag))) break;
-              mbar_arrive(&bars->empty[x % NS]);
+              if (!(ok = wait_warp(&bars->full[x % NS], (x / NS) & 1, abort_flag))) break;
+              if (lane == 0) mbar_arrive(&bars->empty[x % NS]);
             }
-            mbar_arrive(&bars->q_empty);
+            if (lane == 0) mbar_arrive(&bars->q_empty);
           } else {
             // S of half j into buffer j & 1, which P V of half j - 2 has left
             auto issue_s = [&](int j) -> bool {
               const int item = items + 2 * (j >> 1), st = item % NS, h = j & 1;
-              if (h == 0 && !mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag)) return false;
+              if (h == 0 && !wait_warp(&bars->full[st], (item / NS) & 1, abort_flag)) return false;
               tc_fence_after();
+              const uint64_t k_desc = sw128_desc(ring + st * L::TILE + h * kHalfKeys * 128, 16, 1024);
+              if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-                mma_f16_ss(s_col + h * kHalfKeys, sw128_desc(q_base + o, 16, 1024),
-                           sw128_desc(ring + st * L::TILE + o + h * kHalfKeys * 128, 16, 1024), IDESC_QK, kk > 0);
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                  const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+                  mma_f16_ss(s_col + h * kHalfKeys, desc_at(q_desc, o), desc_at(k_desc, o), IDESC_QK, kk > 0);
+                }
+                mma_commit(&bars->s_full[q][h]);
+                if (h == 1) mma_commit(&bars->empty[st]);
+                if (j == 2 * nt - 1) mma_commit(&bars->q_empty);
               }
-              mma_commit(&bars->s_full[q][h]);
-              if (h == 1) mma_commit(&bars->empty[st]);
-              if (j == 2 * nt - 1) mma_commit(&bars->q_empty);
+              __syncwarp();
               return true;
             };
             ok = ok && issue_s(0) && issue_s(1);
             for (int j = 0; j < 2 * nt && ok; ++j, ++jj) {
               const int item = items + 2 * (j >> 1) + 1, st = item % NS, h = j & 1;
-              if (h == 0 && !(ok = mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag))) break;
-              if (j == 0 && !(ok = mbar_wait(&bars->o_empty[q], (mine & 1) ^ 1, abort_flag))) break;
-              if (!(ok = mbar_wait(&bars->p_full[q][h], (jj >> 1) & 1, abort_flag))) break;
+              if (h == 0 && !(ok = wait_warp(&bars->full[st], (item / NS) & 1, abort_flag))) break;
+              if (j == 0 && !(ok = wait_warp(&bars->o_empty[q], (mine & 1) ^ 1, abort_flag))) break;
+              if (!(ok = wait_warp(&bars->p_full[q][h], (jj >> 1) & 1, abort_flag))) break;
               tc_fence_after();
+              const uint64_t v_desc = sw128_desc(ring + st * L::TILE + h * kHalfKeys * 128, kHalf, 1024);
+              if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < kHalfKeys / 16; ++kk)
-                mma_f16_ts(o_col, s_col + h * kHalfKeys + kk * 8,
-                           sw128_desc(ring + st * L::TILE + (h * kHalfKeys + kk * 16) * 128, kHalf, 1024), IDESC_PV,
-                           j > 0 || kk > 0);
-              mma_commit(&bars->pv_done[q]);
-              if (h == 1) mma_commit(&bars->empty[st]);
+                for (int kk = 0; kk < kHalfKeys / 16; ++kk)
+                  mma_f16_ts(o_col, s_col + h * kHalfKeys + kk * 8, desc_at(v_desc, kk * 16 * 128), IDESC_PV, j > 0 || kk > 0);
+                mma_commit(&bars->pv_done[q]);
+                if (h == 1) mma_commit(&bars->empty[st]);
+              }
+              __syncwarp();
               if (j + 2 < 2 * nt) ok = issue_s(j + 2);
             }
             ++mine;
