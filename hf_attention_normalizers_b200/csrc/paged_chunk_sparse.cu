@@ -213,29 +213,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp > 8) {
     // ------------------------------------------------------------ MMA issuers
     const int q = warp - 9;
-    if (lane == 0 && q < nact && nt > 0) {
-      const uint32_t q_base = smem_u32(smem + q * L::TILE), k_base = smem_u32(smem + L::K);
-      bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
+    if (q < nact && nt > 0) {
+      const uint64_t q_desc = sw128_desc(smem_u32(smem + q * L::TILE), 16, 1024);
+      const uint32_t k_base = smem_u32(smem + L::K);
+      bool ok = wait_warp(&bars->q_full, 0, abort_flag);
       int it = 0;
       for (int pass = 0; ok; ++pass) {
         for (int t = 0; t < nt; ++t, ++it) {
           const int st = it % NS, sb = it & 1;
-          if (!(ok = mbar_wait(&bars->full[st], (it / NS) & 1, abort_flag))) break;
-          if (!(ok = mbar_wait(&bars->s_empty[q][sb], ((it >> 1) & 1) ^ 1, abort_flag))) break;
+          if (!(ok = wait_warp(&bars->full[st], (it / NS) & 1, abort_flag))) break;
+          if (!(ok = wait_warp(&bars->s_empty[q][sb], ((it >> 1) & 1) ^ 1, abort_flag))) break;
           tc_fence_after();
+          const uint64_t k_desc = sw128_desc(k_base + st * L::TILE, 16, 1024);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-            mma_f16_ss(tmem + (2 * q + sb) * 128, sw128_desc(q_base + o, 16, 1024),
-                       sw128_desc(k_base + st * L::TILE + o, 16, 1024), IDESC, kk > 0);
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+              mma_f16_ss(tmem + (2 * q + sb) * 128, desc_at(q_desc, o), desc_at(k_desc, o), IDESC, kk > 0);
+            }
+            mma_commit(&bars->s_full[q][sb]);
+            mma_commit(&bars->empty[st]);
           }
-          mma_commit(&bars->s_full[q][sb]);
-          mma_commit(&bars->empty[st]);
+          __syncwarp();
         }
-        if (!ok || !(ok = mbar_wait(&bars->ctrl, pass & 1, abort_flag))) break;
+        if (!ok || !(ok = wait_warp(&bars->ctrl, pass & 1, abort_flag))) break;
         if (!*(volatile int*)&bars->again) break;
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         fail(p, bars);
         mma_commit(&bars->drain[q]);
         mbar_wait(&bars->drain[q], 0, &bars->never);

@@ -533,24 +533,28 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
     __syncwarp();
   } else if (warp > 8) {
     const int w = warp - 9;
-    if (lane == 0 && w < nt) {
-      const uint32_t k_base = smem_u32(smem), q_base = smem_u32(smem + L::Q + w * L::TILE);
-      bool ok = mbar_wait(&bars->k_full, 0, abort_flag);
+    if (w < nt) {
+      const uint64_t k_desc = sw128_desc(smem_u32(smem), 16, 1024);
+      const uint64_t q_desc = sw128_desc(smem_u32(smem + L::Q + w * L::TILE), 16, 1024);
+      bool ok = wait_warp(&bars->k_full, 0, abort_flag);
       for (int u = w; u < nt && ok; u += 2) {
         const int ph = (u >> 1) & 1;
-        if (!(ok = mbar_wait(&bars->q_full[w], ph, abort_flag))) break;
-        if (!(ok = mbar_wait(&bars->s_empty[w], ph ^ 1, abort_flag))) break;
+        if (!(ok = wait_warp(&bars->q_full[w], ph, abort_flag))) break;
+        if (!(ok = wait_warp(&bars->s_empty[w], ph ^ 1, abort_flag))) break;
         tc_fence_after();
         const uint32_t idesc = idesc_f16(BF16, 128, (rows_of(t_lo + u) + 15) & ~15, false, false);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
-          mma_f16_ss(tmem + w * 128, sw128_desc(k_base + o, 16, 1024), sw128_desc(q_base + o, 16, 1024), idesc, kk > 0);
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t o = (kk >> 2) * kHalf + (kk & 3) * 32;
+            mma_f16_ss(tmem + w * 128, desc_at(k_desc, o), desc_at(q_desc, o), idesc, kk > 0);
+          }
+          mma_commit(&bars->s_full[w]);
+          mma_commit(&bars->q_empty[w]);
         }
-        mma_commit(&bars->s_full[w]);
-        mma_commit(&bars->q_empty[w]);
+        __syncwarp();
       }
-      if (!ok) {
+      if (!ok && lane == 0) {
         fail(p, ctl);
         mma_commit(&bars->drain[w]);
         mbar_wait(&bars->drain[w], 0, &ctl->never);

@@ -161,49 +161,50 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     bool ok = true;
     int it = 0, pieces = 0;
     const uint32_t base = smem_u32(smem);
-    auto issue_s = [&](int i, int qb) -> bool {
+    auto issue_s = [&](int i, int qb, bool last) -> bool {
       const int item = 2 * i, st = item % NS, sb = i & 1;
-      if (!mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag)) return false;
-      if (!mbar_wait(&bars->s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag)) return false;
+      if (!wait_warp(&bars->full[st], (item / NS) & 1, abort_flag)) return false;
+      if (!wait_warp(&bars->s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag)) return false;
       tc_fence_after();
+      const uint64_t k_desc = sw128_desc(base + st * L::TILE, 16, 1024), q_desc = sw128_desc(base + L::Q + qb * L::QB, 16, 1024);
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk)
-        mma_f16_ss(tmem + sb * NC, sw128_desc(base + st * L::TILE + (kk >> 2) * kHalf + (kk & 3) * 32, 16, 1024),
-                   sw128_desc(base + L::Q + qb * L::QB + (kk >> 2) * NC * 128 + (kk & 3) * 32, 16, 1024), IDESC_QK, kk > 0);
-      mma_commit(&bars->s_full[sb]);
-      mma_commit(&bars->empty[st]);
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_f16_ss(tmem + sb * NC, desc_at(k_desc, (kk >> 2) * kHalf + (kk & 3) * 32),
+                     desc_at(q_desc, (kk >> 2) * NC * 128 + (kk & 3) * 32), IDESC_QK, kk > 0);
+        mma_commit(&bars->s_full[sb]);
+        mma_commit(&bars->empty[st]);
+        if (last) mma_commit(&bars->q_empty[qb]);
+      }
+      __syncwarp();
       return true;
     };
     while (walk.next()) {
-      if (lane == 0 && ok) {
-        const int nt = walk.piece.nt, qb = pieces & 1;
-        ok = mbar_wait(&bars->q_full[qb], (pieces >> 1) & 1, abort_flag) && issue_s(it, qb);
-        if (ok && nt == 1) mma_commit(&bars->q_empty[qb]);
-        for (int t = 0; t < nt && ok; ++t, ++it) {
-          if (t + 1 < nt) {
-            if (!(ok = issue_s(it + 1, qb))) break;
-            if (t + 2 == nt) mma_commit(&bars->q_empty[qb]);
-          }
-          const int item = 2 * it + 1, st = item % NS, pb = it & 1;
-          if (t == 0 && !(ok = mbar_wait(&bars->o_empty, (pieces & 1) ^ 1, abort_flag))) break;
-          if (!(ok = mbar_wait(&bars->full[st], (item / NS) & 1, abort_flag))) break;
-          if (!(ok = mbar_wait(&bars->p_full[pb], (it >> 1) & 1, abort_flag))) break;
-          tc_fence_after();
+      const int nt = walk.piece.nt, qb = pieces & 1;
+      if (ok) ok = wait_warp(&bars->q_full[qb], (pieces >> 1) & 1, abort_flag) && issue_s(it, qb, nt == 1);
+      for (int t = 0; t < nt && ok; ++t, ++it) {
+        if (t + 1 < nt && !(ok = issue_s(it + 1, qb, t + 2 == nt))) break;
+        const int item = 2 * it + 1, st = item % NS, pb = it & 1;
+        if (t == 0 && !(ok = wait_warp(&bars->o_empty, (pieces & 1) ^ 1, abort_flag))) break;
+        if (!(ok = wait_warp(&bars->full[st], (item / NS) & 1, abort_flag))) break;
+        if (!(ok = wait_warp(&bars->p_full[pb], (it >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        const uint64_t v_desc = sw128_desc(base + st * L::TILE, kHalf, 1024), p_desc = sw128_desc(base + L::P + pb * L::PB, 16, 1024);
+        if (elect_one()) {
           // A = V^T: rows of the tile are keys (the K axis), head dims contiguous;
           // at HD = 64 rows 64 .. 127 of the product come from the bytes after
           // the tile and are not read
 #pragma unroll
           for (int kk = 0; kk < kTileKeys / 16; ++kk)
-            mma_f16_ss(tmem + 2 * NC, sw128_desc(base + st * L::TILE + kk * 16 * 128, kHalf, 1024),
-                       sw128_desc(base + L::P + pb * L::PB + (kk >> 2) * NC * 128 + (kk & 3) * 32, 16, 1024), IDESC_PV,
-                       t > 0 || kk > 0);
+            mma_f16_ss(tmem + 2 * NC, desc_at(v_desc, kk * 16 * 128), desc_at(p_desc, (kk >> 2) * NC * 128 + (kk & 3) * 32),
+                       IDESC_PV, t > 0 || kk > 0);
           mma_commit(&bars->empty[st]);
           mma_commit(&bars->p_empty[pb]);
           if (t + 1 == nt) mma_commit(&bars->o_full);
         }
-        ++pieces;
+        __syncwarp();
       }
-      __syncwarp();
+      ++pieces;
     }
     if (lane == 0 && !ok) {
       fail(p, bars);
