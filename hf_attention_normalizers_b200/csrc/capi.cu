@@ -288,6 +288,8 @@ int fill_chunk(const hfan_chunk_desc* desc, AttnParams& p) {
     return fail(HFAN_ERR_INVALID, "block_table and sequence_lengths are required");
   if (desc->total_q < 0 || desc->max_len_q < 0 || desc->max_len_k < 0 || desc->num_cache_tokens < 0)
     return fail(HFAN_ERR_INVALID, "negative length");
+  if (desc->num_cache_tokens > 2147483647ll)
+    return fail(HFAN_ERR_INVALID, "more than 2^31 - 1 cache slots are not supported");
   if ((int64_t)desc->total_q * desc->heads_q > 2147483647ll)
     return fail(HFAN_ERR_INVALID, "more than 2^31 - 1 (token, head) rows in one call");
   if ((int64_t)desc->max_blocks * desc->page_size < desc->max_len_k)

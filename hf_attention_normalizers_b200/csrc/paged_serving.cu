@@ -4,6 +4,7 @@
 #include "common.cuh"
 #include "params.cuh"
 #include "paged_serving.cuh"
+#include "paged_walk.cuh"
 
 namespace hfan {
 namespace {
@@ -37,6 +38,23 @@ __global__ void __launch_bounds__(256) append_kernel(AttnParams p, const U* k, c
   }
 }
 
+// Cache rows of a sequence's positions; `shift`: log2 of the page size, or -1.
+struct Rows {
+  const int* table;
+  int page_size, shift;
+  int64_t tokens;
+  int* status;
+  __device__ __forceinline__ int operator()(int pos) const {
+    const int page = table[shift >= 0 ? pos >> shift : pos / page_size];
+    const int64_t row = (int64_t)page * page_size + (shift >= 0 ? pos & (page_size - 1) : pos % page_size);
+    if (page < 0 || row >= tokens) {
+      if (status) atomicCAS(status, kDevOk, kDevBadPage);
+      return -1;
+    }
+    return (int)row;
+  }
+};
+
 // ---------------------------------------------------------------------------
 // evict, selection: one CTA per (sequence, KV head).  The weights of the
 // positions before the `recent` last ones are ranked by a radix selection on
@@ -60,15 +78,16 @@ __device__ __forceinline__ uint32_t rank_bits(float f) {
 __device__ __forceinline__ int warp_sum_int(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(AttnParams p, const float* kw, int64_t ldw, int budget,
-                                                                   int recent, int* kept, int* new_lens, int cache) {
+                                                                   int recent, int page_shift, int* kept, int* new_lens,
+                                                                   int cache) {
+  tc::allow_dependents();
   extern __shared__ uint32_t img[];  // [cache] images of the weights
   __shared__ int hist[kBins];
   __shared__ int wsum[2][kSelWarps];
   __shared__ int found[2];
   const int h = blockIdx.x, b = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Geometry g;
-  g.k_start = 0;
+  const Rows rows{p.block_table + (int64_t)b * p.max_blocks, p.page_size, page_shift, p.num_cache_tokens, p.dev_status};
   const int L = seq_len_k(p, b);
   int* out = kept + ((int64_t)b * p.hkv + h) * budget;
   if (h == 0 && threadIdx.x == 0) new_lens[b] = min(L, budget);
@@ -79,10 +98,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(AttnParams p,
   const int late = min(recent, budget), cand = L - late, want = budget - late;  // want < cand
   const float* w = kw + (int64_t)h * ldw;
   auto fetch = [&](int j) -> uint32_t {
-    const int64_t tok = key_token(p, g, b, j);
+    const int tok = rows(j);
     return tok < 0 ? 0u : rank_bits(w[tok]);
   };
   const int held = min(cand, cache);
+#pragma unroll 4
   for (int j = threadIdx.x; j < held; j += kSelThreads) img[j] = fetch(j);
   auto image = [&](int j) -> uint32_t { return j < held ? img[j] : fetch(j); };
 
@@ -166,63 +186,66 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(AttnParams p,
 // ---------------------------------------------------------------------------
 // evict, move: kept position kept[i] >= i goes to logical position i.  One CTA
 // owns a strip (some columns of K, of V, or the weights) of one (sequence, KV
-// head), so strips are independent; within a strip the rows go in steps of
-// kRowsStep in increasing order.  A step reads rows kept[i] >= i of its own i
-// range, so only its own writes can hit its reads: one barrier between the
-// loads and the stores of a step, and the next step's loads (rows beyond
-// every row written so far) need none.
+// head), so strips are independent; within a strip the rows go in steps, in
+// increasing order.  A step reads rows kept[i] >= i of its own i range, so only
+// its own writes can hit its reads: one barrier between the loads and the
+// stores of a step, and the loads of the next one (rows beyond every row
+// written so far) are in flight before them.
+//
+// Bound by memory: each kept row is read and written once.  Strips are whole
+// rows when there are enough (sequence, head) pairs to fill the SMs; else they
+// get narrower, down to a 32-byte sector, since a strip goes at the pace of one
+// load after the other.  32 sequences of 16k keys cut to 4k (1.07 GB): 265 us,
+// 4.0 TB/s -- the 256-byte rows lie scattered over the pages; more rows in
+// flight per thread were slower (four: 300 us, eight: 440), 256 threads too
+// (380), and narrow strips no faster (270).
 // ---------------------------------------------------------------------------
-constexpr int kMoveIlp = 4;
+constexpr int kMoveThreads = 512;
 
 template <typename U>
-__device__ void move_strip(const AttnParams& p, int b, const int* kept, int count, U* base, int64_t st, int width,
-                           int lanes) {
-  Geometry g;
-  g.k_start = 0;
-  const int rows = blockDim.x / lanes;  // rows of one load each
-  const int c = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
-  const bool on = r0 < rows && c < width;
-  for (int i0 = 0; i0 < count; i0 += rows * kMoveIlp) {
-    U val[kMoveIlp];
-    int64_t dst[kMoveIlp];
-#pragma unroll
-    for (int e = 0; e < kMoveIlp; ++e) {
-      const int i = i0 + e * rows + r0;
-      dst[e] = -1;
-      if (on && i < count) {
-        const int j = kept[i];
-        if (j != i) {
-          const int64_t src = key_token(p, g, b, j);
-          if (src >= 0) {
-            dst[e] = key_token(p, g, b, i);
-            val[e] = base[src * st + c];
-          }
-        }
-      }
-    }
+__device__ void move_strip(const Rows& rows, const int* kept, int count, U* base, int64_t st, int width, int lanes) {
+  const int step = kMoveThreads / lanes, c = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
+  const bool on = r0 < step && c < width;
+  auto load = [&](int i, U& v) -> int {  // the row that v goes to, or -1
+    if (!on || i >= count) return -1;
+    const int j = kept[i];
+    if (j == i) return -1;
+    const int src = rows(j);
+    if (src < 0) return -1;
+    v = base[(int64_t)src * st + c];
+    return rows(i);
+  };
+  U v0, v1;
+  int d0 = load(r0, v0);
+  for (int i0 = 0; i0 < count; i0 += 2 * step) {
+    const int d1 = load(i0 + step + r0, v1);
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kMoveIlp; ++e)
-      if (dst[e] >= 0) base[dst[e] * st + c] = val[e];
+    if (d0 >= 0) base[(int64_t)d0 * st + c] = v0;
+    d0 = load(i0 + 2 * step + r0, v0);
+    __syncthreads();
+    if (d1 >= 0) base[(int64_t)d1 * st + c] = v1;
   }
 }
 
 template <typename U>
-__global__ void __launch_bounds__(256) evict_move_kernel(AttnParams p, U* kc, U* vc, float* kw, int64_t ldw, int units,
-                                                         int slice, int slices, int budget, const int* kept) {
+__global__ void __launch_bounds__(kMoveThreads, 4) evict_move_kernel(AttnParams p, U* kc, U* vc, float* kw, int64_t ldw,
+                                                                  int units, int slice, int slices, int budget,
+                                                                  int page_shift, const int* kept) {
+  tc::wait_for_predecessor();
   const int h = blockIdx.y, b = blockIdx.z;
   const int L = seq_len_k(p, b);
   if (L <= budget) return;
   const int* kp = kept + ((int64_t)b * p.hkv + h) * budget;
+  const Rows rows{p.block_table + (int64_t)b * p.max_blocks, p.page_size, page_shift, p.num_cache_tokens, p.dev_status};
   const int s = blockIdx.x;
   if (s == 2 * slices) {
-    move_strip<float>(p, b, kp, budget, kw + (int64_t)h * ldw, 1, 1, 1);
+    move_strip<float>(rows, kp, budget, kw + (int64_t)h * ldw, 1, 1, 1);
   } else {
     const int c0 = (s % slices) * slice, width = min(slice, units - c0);
     if (s < slices)
-      move_strip<U>(p, b, kp, budget, kc + (int64_t)h * p.k_sh + c0, p.k_st, width, slice);
+      move_strip<U>(rows, kp, budget, kc + (int64_t)h * p.k_sh + c0, p.k_st, width, slice);
     else
-      move_strip<U>(p, b, kp, budget, vc + (int64_t)h * p.v_sh + c0, p.v_st, width, slice);
+      move_strip<U>(rows, kp, budget, vc + (int64_t)h * p.v_sh + c0, p.v_st, width, slice);
   }
 }
 
@@ -263,6 +286,8 @@ __global__ void __launch_bounds__(256) key_weights_kernel(AttnParams p, float* k
   if (lane == 0 && acc != 0.f) atomicAdd(kw + (int64_t)kvh * ldw + tok, acc);
 }
 
+int page_shift(const AttnParams& p) { return (p.page_size & (p.page_size - 1)) == 0 ? __builtin_ctz(p.page_size) : -1; }
+
 int elem_bytes(int dtype) { return dtype == HFAN_FLOAT32 ? 4 : 2; }
 
 bool vec16(const void* ptr, int64_t a, int64_t b, int es) {
@@ -290,12 +315,16 @@ cudaError_t move_t(int dtype, const AttnParams& p0, float* kw, int64_t ldw, int 
   AttnParams p = p0;
   const int per = (int)sizeof(U) / elem_bytes(dtype), units = p.d / per;
   p.k_st /= per; p.k_sh /= per; p.v_st /= per; p.v_sh /= per;
-  const int slice = sizeof(U) == 16 ? (units < 4 ? units : 4) : (units < 32 ? units : 32);
+  // vectors of a strip's row: the whole row, halved while the strips would not
+  // give every SM two CTAs, but no less than a sector
+  const int sector = 32 / (int)sizeof(U);
+  int slice = units < 64 ? units : 64;
+  while (slice % 2 == 0 && slice / 2 >= sector && (int64_t)p.batch * p.hkv * 2 * ((units + slice - 1) / slice) < 2 * sm_count())
+    slice /= 2;
   const int slices = (units + slice - 1) / slice;
-  evict_move_kernel<U><<<dim3(2 * slices + 1, p.hkv, p.batch), 256, 0, s>>>(
-      p, static_cast<U*>(const_cast<void*>(p.k)), static_cast<U*>(const_cast<void*>(p.v)), kw, ldw, units, slice, slices,
-      budget, kept);
-  return cudaGetLastError();
+  return launch_dependent(evict_move_kernel<U>, dim3(2 * slices + 1, p.hkv, p.batch), kMoveThreads, s, p,
+                          static_cast<U*>(const_cast<void*>(p.k)), static_cast<U*>(const_cast<void*>(p.v)), kw, ldw, units,
+                          slice, slices, budget, page_shift(p), kept);
 }
 
 }  // namespace
@@ -317,7 +346,8 @@ cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw
         cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelCache * 4);
     if (e != cudaSuccess) return e;
   }
-  evict_select_kernel<<<dim3(p.hkv, p.batch), kSelThreads, smem, s>>>(p, kw, ldw, budget, recent, kept, new_lens, cache);
+  evict_select_kernel<<<dim3(p.hkv, p.batch), kSelThreads, smem, s>>>(p, kw, ldw, budget, recent, page_shift(p), kept, new_lens,
+                                                                                cache);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.len_k <= budget) return e;
   const int es = elem_bytes(dtype);

@@ -61,6 +61,7 @@ def _desc(**kw):
     (dict(cu_seqlens_q=None), "cu_seqlens_q"),
     (dict(total_q=-1), "negative"),
     (dict(total_q=2 ** 30), "rows in one call"),
+    (dict(num_cache_tokens=2 ** 31), "cache slots"),
 ])
 def test_requests_are_refused_on_the_host(kw, msg):
     lib, t = N.lib(), N.HfanTensor(None, 0, 0, 0)
