@@ -31,7 +31,8 @@ capacity are taken, which costs idle thread blocks.
 
 from __future__ import annotations
 
-from typing import Callable, Optional, Union
+from dataclasses import dataclass
+from typing import Callable, Optional, Sequence, Union
 
 import torch
 
@@ -39,7 +40,7 @@ from . import _native as N
 from . import ops
 from .paged import _normalizer_name
 
-__all__ = ["paged_append", "paged_chunk_attention", "paged_evict", "device_status"]
+__all__ = ["PagedServingCache", "paged_append", "paged_chunk_attention", "paged_evict", "device_status"]
 
 
 _INTS = (torch.int32, torch.int64)
@@ -187,3 +188,93 @@ def device_status(clear: bool = True) -> int:
     """Wait for the current stream and read the device status word: 0, or the first error the kernels
     recorded (1: page id outside the cache, 2: a bounded wait ran out, 3: length or offset out of range)."""
     return N.device_status(torch.cuda.current_stream().cuda_stream, clear)
+
+
+@dataclass
+class ServingStep:
+    """One step of a batch, as ``PagedServingCache.step`` laid it out (device tensors and their host bounds)."""
+
+    block_table: torch.Tensor
+    cu_seqlens: torch.Tensor
+    lengths: torch.Tensor
+    max_seqlen_q: int
+    max_seqlen_k: int
+
+
+class PagedServingCache:
+    """The pages of a batch over all layers, with their bookkeeping on the host.
+
+    ``step`` gives every sequence room for its new tokens; ``append`` and
+    ``attend`` are called once per layer of that step; ``evict`` cuts every
+    sequence to a budget and returns the freed pages.  Lengths follow from what
+    the host has asked for, so no call waits for the GPU.
+    """
+
+    def __init__(self, num_layers: int, num_sequences: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, device: Union[str, torch.device] = "cuda", track_weights: bool = False):
+        slots = num_blocks * block_size
+        # K and V of a slot side by side: one allocation a layer
+        self.layers = [torch.zeros(slots, 2, kv_heads, head_dim, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.weights = [torch.zeros(kv_heads, slots, device=device) if track_weights else None for _ in range(num_layers)]
+        self.block_size = block_size
+        self.lengths = [0] * num_sequences
+        self._pages: list[list[int]] = [[] for _ in range(num_sequences)]
+        self._free = list(range(num_blocks - 1, -1, -1))
+        self._device = torch.device(device)
+
+    def step(self, new_tokens: Sequence[int]) -> ServingStep:
+        """Allocate pages for ``new_tokens[b]`` more tokens of every sequence (0: the sequence rests)."""
+        if len(new_tokens) != len(self.lengths):
+            raise ValueError("new_tokens must have one count per sequence.")
+        if any(n < 0 for n in new_tokens):
+            raise ValueError("new_tokens must not be negative.")
+        need = [-(-(c + n) // self.block_size) - len(p) for c, n, p in zip(self.lengths, new_tokens, self._pages)]
+        if sum(max(n, 0) for n in need) > len(self._free):
+            raise ValueError("The cache has no room for the new tokens.")
+        for b, n in enumerate(need):
+            self._pages[b].extend(self._free.pop() for _ in range(n))
+            self.lengths[b] += new_tokens[b]
+        return self._describe(new_tokens)
+
+    def _describe(self, new_tokens: Sequence[int]) -> ServingStep:
+        width = max(1, max(len(p) for p in self._pages))
+        offsets = [0]
+        for n in new_tokens:
+            offsets.append(offsets[-1] + n)
+        host = offsets + self.lengths
+        for p in self._pages:
+            host = host + p + [0] * (width - len(p))
+        flat = torch.tensor(host, dtype=torch.int32)
+        if self._device.type == "cuda":
+            flat = flat.pin_memory().to(self._device, non_blocking=True)
+        b = len(self.lengths)
+        return ServingStep(flat[2 * b + 1:].view(b, width), flat[:b + 1], flat[b + 1:2 * b + 1], max(new_tokens),
+                           max(self.lengths))
+
+    def append(self, layer: int, step: ServingStep, key: torch.Tensor, value: torch.Tensor) -> None:
+        kv = self.layers[layer]
+        paged_append(key, value, kv[:, 0], kv[:, 1], step.block_table, step.cu_seqlens, step.lengths, self.block_size,
+                     key_weights=self.weights[layer])
+
+    def attend(self, layer: int, step: ServingStep, query: torch.Tensor,
+               normalizer: Union[str, Callable[..., torch.Tensor]] = "softmax1", scale: Optional[float] = None) -> torch.Tensor:
+        kv = self.layers[layer]
+        return paged_chunk_attention(query, kv[:, 0], kv[:, 1], step.block_table, step.cu_seqlens, step.lengths,
+                                     self.block_size, normalizer, scale, key_weights=self.weights[layer],
+                                     max_seqlen_q=step.max_seqlen_q, max_seqlen_k=step.max_seqlen_k)
+
+    def evict(self, budget: int, recent: int = 0) -> None:
+        """Cut every sequence longer than ``budget`` in all layers and free the pages that this empties."""
+        if any(w is None for w in self.weights):
+            raise ValueError("evict needs a cache made with track_weights=True.")
+        if max(self.lengths) <= budget:
+            return
+        step = self._describe([0] * len(self.lengths))
+        for kv, w in zip(self.layers, self.weights):
+            paged_evict(kv[:, 0], kv[:, 1], w, step.block_table, step.lengths, self.block_size, budget, recent=recent,
+                        max_seqlen_k=step.max_seqlen_k)
+        for b, c in enumerate(self.lengths):
+            self.lengths[b] = min(c, budget)
+            keep = -(-self.lengths[b] // self.block_size)
+            self._free.extend(reversed(self._pages[b][keep:]))
+            del self._pages[b][keep:]

@@ -448,3 +448,80 @@ def test_tensors_elsewhere_are_refused():
         serving.paged_chunk_attention(b.query, b.key_cache, b.value_cache, b.table, b.cu, b.seq, b.page)
     with pytest.raises(ValueError, match="one device"):
         serving.paged_chunk_attention(b.d_query, b.d_key, b.d_value, b.table, b.d_cu, b.d_seq, b.page)
+
+
+# ---------------------------------------------------------------------------
+# the cache and the example, as a user runs them
+# ---------------------------------------------------------------------------
+def _example():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_paged.py")
+    spec = importlib.util.spec_from_file_location("serve_paged", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_serving_a_model_matches_its_full_forward(norm):
+    """Prompt pieces and single tokens through the pages give the logits of one pass over the whole text.
+
+    Both run in bfloat16 through the same layers; only the attention's own rounding differs, a few units of 2^-8
+    of a hidden state whose logits have unit scale.
+    """
+    import hf_attention_normalizers_b200 as H
+
+    ex = _example()
+    model = ex.small_model(layers=2)
+    texts = [torch.randint(0, 1024, (n,), generator=torch.Generator().manual_seed(n)).tolist() for n in (150, 37, 1)]
+    plan = [[64, 37, 0], [64, 0, 1], [21, 0, 0], [1, 0, 0]]
+    c = model.config
+    cache = serving.PagedServingCache(2, 3, 12, 32, c.num_key_value_heads, c.head_dim)
+    got = [[], [], []]
+    with torch.no_grad():
+        at = [0, 0, 0]
+        for counts in plan:
+            step = cache.step(counts)
+            ids = torch.tensor([t for s, p, n in zip(texts, at, counts) for t in s[p:p + n]], device="cuda")
+            pos = torch.tensor([p + i for p, n in zip(at, counts) for i in range(n)], device="cuda")
+            logits = ex.forward_step(model, cache, step, ids, pos, norm).float()
+            for b, part in enumerate(logits.split(counts)):
+                got[b].append(part)
+                at[b] += counts[b]
+        H.set_softmax_attention_backend(model, base_backend="sdpa", softmax_fn=norm)
+        for text, parts in zip(texts, got):
+            want = model(torch.tensor([text], device="cuda")).logits[0].float()
+            have = torch.cat(parts)
+            assert have.shape == want.shape
+            assert (have - want).norm() <= 2.0 ** -5 * want.norm()
+
+
+@pytest.mark.parametrize("norm", NORMS)
+def test_serving_under_a_budget_frees_pages(norm):
+    ex = _example()
+    model = ex.small_model(layers=2)
+    prompts = [list(range(300)), list(range(40)), [5]]
+    free = ex.generate(model, prompts, 6, norm, piece=64)
+    # a budget that nothing exceeds changes nothing; a small one runs in the memory of the budget alone
+    assert ex.generate(model, prompts, 6, norm, piece=64, budget=400) == free
+    cut = ex.generate(model, prompts, 6, norm, piece=64, budget=96, recent=16)
+    assert [len(o) for o in cut] == [6, 6, 6] and serving.device_status() == 0
+
+
+def test_cache_bookkeeping():
+    cache = serving.PagedServingCache(1, 2, 6, 16, 1, 64, track_weights=True)
+    step = cache.step([40, 16])
+    assert cache.lengths == [40, 16] and step.max_seqlen_q == 40 and step.max_seqlen_k == 40
+    assert step.cu_seqlens.tolist() == [0, 40, 56] and step.lengths.tolist() == [40, 16]
+    with pytest.raises(ValueError, match="no room"):
+        cache.step([40, 16])
+    with pytest.raises(ValueError, match="one count per sequence"):
+        cache.step([1])
+    cache.evict(20, 4)
+    assert cache.lengths == [20, 16]
+    step = cache.step([12, 33])  # 32 and 49 tokens: six pages again
+    assert cache.lengths == [32, 49] and len(set(step.block_table[0, :2].tolist() + step.block_table[1, :4].tolist())) == 6
+    with pytest.raises(ValueError, match="track_weights"):
+        serving.PagedServingCache(1, 1, 2, 16, 1, 64).evict(4)
