@@ -8,12 +8,15 @@ names the cause.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 _LIB_PATH = os.environ.get("HFAN_LIBRARY") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libhfan.so")
+_BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_hfan_torch.so")
 _lock = threading.Lock()
 _lib = None
+_binding = None
 
 SOFTMAX1, SPARSEMAX, ENTMAX15 = 0, 1, 2
 FLOAT32, FLOAT16, BFLOAT16 = 0, 1, 2
@@ -155,6 +158,30 @@ def lib():
                 raise RuntimeError("hfan native library ABI version mismatch; rebuild it")
             _lib = handle
     return _lib
+
+
+def binding():
+    """Load (once) and return the module of the serving calls' host path (``csrc/torch_binding.cpp``), bound to ``lib()``."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    handle = lib()
+    with _lock:
+        if _binding is None:
+            if not os.path.exists(_BINDING_PATH):
+                raise RuntimeError(
+                    f"hfan torch binding not found at {_BINDING_PATH}; build it with "
+                    "`python -m hf_attention_normalizers_b200.build`")
+            import torch  # noqa: F401  (its libraries resolve the module's symbols)
+
+            spec = importlib.util.spec_from_file_location("_hfan_torch", _BINDING_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
+                "hfan_paged_append", "hfan_paged_chunk_workspace_bytes", "hfan_paged_chunk_fwd", "hfan_paged_evict",
+                "hfan_last_error")))
+            _binding = module
+    return _binding
 
 
 def check(rc: int, what: str) -> None:

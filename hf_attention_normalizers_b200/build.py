@@ -1,4 +1,6 @@
-"""Build the native library ``_lib/libhfan.so`` in-tree with nvcc for sm_100a.
+"""Build the native library ``_lib/libhfan.so`` in-tree with nvcc for sm_100a,
+and beside it ``_lib/_hfan_torch.so``, the host path of the paged serving calls
+(``csrc/torch_binding.cpp``, g++ against torch's headers).
 
 Usage: ``python -m hf_attention_normalizers_b200.build`` (or ``build()``).
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` (rebuilt when the
@@ -19,6 +21,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "_lib", "libhfan.so")
+BINDING = os.path.join(PKG, "_lib", "_hfan_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,6 +52,29 @@ def _compile(src, verbose=False):
     return obj
 
 
+def _build_binding(verbose=False):
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    if not _stale(BINDING, [src] + _headers()):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in include_paths()), "-I" + os.path.join(cuda, "include"),
+           "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + torch_lib,
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
@@ -56,8 +82,12 @@ def build(verbose: bool = False, force: bool = False) -> str:
     if force:
         for o in glob.glob(os.path.join(BUILD, "*.o")):
             os.remove(o)
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    if force and os.path.exists(BINDING):
+        os.remove(BINDING)
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        binding = ex.submit(_build_binding, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        binding.result()
     if force or _stale(LIB, objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart"]
         if verbose:

@@ -483,98 +483,30 @@ torch.library.register_autograd("hfan::paged_fwd", _paged_backward, setup_contex
 # ---------------------------------------------------------------------------
 # paged serving
 #
-# The plain functions launch the kernels; the custom ops of the same name
-# wrap them for traced graphs.  A decode step makes these calls for every
-# layer, and the op dispatch costs as much host time as the whole launch, so
-# eager callers (serving.py) use the functions.
+# The plain functions launch the kernels (through csrc/torch_binding.cpp: a
+# decode step makes these calls in every layer, and ctypes would cost more than
+# the kernels); the custom ops of the same name wrap them for traced graphs.
+# The op dispatch costs as much host time as the whole launch, so eager callers
+# (serving.py) use the functions.
 # ---------------------------------------------------------------------------
-_Desc, _View = N.ChunkDesc, N.HfanTensor
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _i32(t: Tensor) -> Tensor:
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
-def _rows3(t: Tensor) -> N.HfanTensor:
-    """``_t3`` of a tensor whose innermost stride is known to be one."""
-    s = t.stride()
-    return _View(t.data_ptr(), 0, s[1], s[0])
-
-
-def _elsewhere(t: Tensor) -> bool:
-    """Whether t lives on another device than the current one (the launch then needs a device guard)."""
-    return t.get_device() != torch.cuda.current_device()
-
-
 def launch_paged_append(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: Tensor, block_table: Tensor,
                         cu_seqlens: Tensor, seq_lens: Tensor, page_size: int, max_q: int,
                         key_weights: Optional[Tensor]) -> None:
-    if _elsewhere(key):
-        with torch.cuda.device(key.device):
-            return launch_paged_append(key, value, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size,
-                                       max_q, key_weights)
-    key, value = _inner_contig(key), _inner_contig(value)
-    bt, cu, sl = _i32(block_table), _i32(cu_seqlens), _i32(seq_lens)
-    total, hkv, d = key.shape
-    batch, cols = bt.shape
-    desc = _Desc(dtype_id(key), N.SOFTMAX1, batch, hkv, hkv, d, total, max_q, page_size, cols, cols * page_size,
-                 key_cache.shape[0], bt.data_ptr(), cu.data_ptr(), sl.data_ptr(), 1.0, 1)
-    kw, ld = (None, 0) if key_weights is None else (key_weights.data_ptr(), key_weights.stride(0))
-    rc = N.lib().hfan_paged_append(ctypes.byref(desc), _rows3(key), _rows3(value), _rows3(key_cache),
-                                   _rows3(value_cache), kw, ld, _raw_stream(key.get_device()))
-    if rc:
-        N.check(rc, "hfan_paged_append")
+    N.binding().append(key, value, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q, key_weights)
 
 
 def launch_paged_chunk_fwd(q: Tensor, key_cache: Tensor, value_cache: Tensor, block_table: Tensor, cu_seqlens: Tensor,
                            seq_lens: Tensor, page_size: int, max_q: int, max_k: int, normalizer: int, scale: float,
                            causal: bool, key_weights: Optional[Tensor] = None) -> tuple[Tensor, Tensor]:
     """Returns (o [T, Hq, D], stats float32 [2, Hq, T]); adds to ``key_weights`` when it is given."""
-    if _elsewhere(q):
-        with torch.cuda.device(q.device):
-            return launch_paged_chunk_fwd(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q,
-                                          max_k, normalizer, scale, causal, key_weights)
-    q = _inner_contig(q)
-    bt, cu, sl = _i32(block_table), _i32(cu_seqlens), _i32(seq_lens)
-    total, hq, d = q.shape
-    batch, cols = bt.shape
-    slots, hkv, _ = key_cache.shape
-    o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    stats = torch.empty((2, hq, total), dtype=torch.float32, device=q.device)
-    desc = _Desc(dtype_id(q), normalizer, batch, hq, hkv, d, total, max_q, page_size, cols, max_k, slots, bt.data_ptr(),
-                 cu.data_ptr(), sl.data_ptr(), scale, causal)
-    kw, ld = (None, 0) if key_weights is None else (key_weights.data_ptr(), key_weights.stride(0))
-    lib, ref = N.lib(), ctypes.byref(desc)
-    nbytes = lib.hfan_paged_chunk_workspace_bytes(ref, kw is not None)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    rc = lib.hfan_paged_chunk_fwd(ref, _rows3(q), _rows3(key_cache), _rows3(value_cache), _rows3(o), stats.data_ptr(), kw, ld,
-                                  None if ws is None else ws.data_ptr(), max(nbytes, 0), _raw_stream(q.get_device()))
-    if rc:
-        N.check(rc, "hfan_paged_chunk_fwd")
-    return o, stats
+    return N.binding().chunk(q, key_cache, value_cache, block_table, cu_seqlens, seq_lens, page_size, max_q, max_k,
+                             normalizer, scale, causal, key_weights)
 
 
 def launch_paged_evict(key_cache: Tensor, value_cache: Tensor, key_weights: Tensor, block_table: Tensor,
                        seq_lens: Tensor, page_size: int, max_k: int, budget: int, recent: int) -> tuple[Tensor, Tensor]:
     """Returns (lengths int32 [B], kept int32 [B, Hkv, budget])."""
-    if _elsewhere(key_cache):
-        with torch.cuda.device(key_cache.device):
-            return launch_paged_evict(key_cache, value_cache, key_weights, block_table, seq_lens, page_size, max_k, budget,
-                                      recent)
-    bt, sl = _i32(block_table), _i32(seq_lens)
-    slots, hkv, d = key_cache.shape
-    batch, cols = bt.shape
-    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=key_cache.device)
-    lens = torch.empty((batch,), dtype=torch.int32, device=key_cache.device)
-    desc = _Desc(dtype_id(key_cache), N.SOFTMAX1, batch, hkv, hkv, d, 0, 0, page_size, cols, max_k, slots, bt.data_ptr(),
-                 None, sl.data_ptr(), 1.0, 1)
-    rc = N.lib().hfan_paged_evict(ctypes.byref(desc), _rows3(key_cache), _rows3(value_cache), key_weights.data_ptr(),
-                                  key_weights.stride(0), budget, recent, kept.data_ptr(), lens.data_ptr(),
-                                  _raw_stream(key_cache.get_device()))
-    if rc:
-        N.check(rc, "hfan_paged_evict")
-    return lens, kept
+    return N.binding().evict(key_cache, value_cache, key_weights, block_table, seq_lens, page_size, max_k, budget, recent)
 
 
 paged_append = torch.library.custom_op(
