@@ -137,6 +137,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = ranks > 1 ? (int)cluster_rank() : 0;
 
+  allow_dependents();
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+  }
+  wait_for_predecessor();
   int b, pair;
   const int unit = blockIdx.x / ranks;
   if (!find_group(p, 2 * c.tpb, unit, &b, &pair)) return;  // the whole cluster alike
@@ -181,7 +187,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ producer
     if (nt > 0) {
       if (lane == 0) {
-        prefetch_tmap(&tm_k);
         mbar_arrive_expect_tx(&bars->q_full, nact * NH * c.tpb * c.group * 128);
         for (int q = 0; q < nact; ++q)
           for (int hh = 0; hh < NH; ++hh)
@@ -574,12 +579,14 @@ cudaError_t run(const AttnParams& p, const ChunkPlan& c, int ranks, int* flags, 
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ranks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  cfg.numAttrs = ranks > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, tq, tk, p, c, ranks, flags);
 }
 

@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     ctl->abort = ctl->never = 0;
     fence_barrier_init();
   }
+  wait_for_predecessor();
   Source src(p, 2 * c.tpb, flags);
   if (!src.any()) return;  // nothing was left to this block
   if (warp == 8) tmem_alloc(&ctl->tmem, 512);
@@ -476,6 +477,8 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
                          const AttnParams p, const ChunkPlan c, float* kw, int64_t ldw) {
   using L = WeightLayout<HD>;
   constexpr int NH = L::NH;
+  allow_dependents();
+  wait_for_predecessor();
   const int b = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * kTileKeys;
   const Geometry g = geometry(p, b);
   if (k0 >= g.k_len || g.q_len == 0) return;
@@ -673,15 +676,16 @@ cudaError_t fwd_t(const AttnParams& p, const ChunkPlan& c, void* workspace, cuda
   if (NORM == HFAN_SOFTMAX1) {
     const int ctas = sm_count();
     const PieceWs ws = piece_ws(p, ctas, kUnitRows, workspace);
-    chunk_fwd_kernel<HD, BF16, NORM><<<ctas, kChunkThreads, smem, s>>>(tq, tk, tv, p, c, ws, nullptr);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, s, p, ws, c.group);
+    e = launch_dependent(chunk_fwd_kernel<HD, BF16, NORM>, dim3(ctas), kChunkThreads, smem, s, tq, tk, tv, p, c, ws,
+                         static_cast<const int*>(nullptr));
+    if (e != cudaSuccess) return e;
+    return launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, 0, s, p, ws, c.group);
   }
   int* flags = static_cast<int*>(workspace);
   e = chunk_sparse_scan(BF16 ? HFAN_BFLOAT16 : HFAN_FLOAT16, p, c, flags, s);
   if (e != cudaSuccess) return e;
-  chunk_fwd_kernel<HD, BF16, NORM><<<dim3(c.pairs, p.hkv), kChunkThreads, smem, s>>>(tq, tk, tv, p, c, PieceWs{}, flags);
-  return cudaGetLastError();
+  return launch_dependent(chunk_fwd_kernel<HD, BF16, NORM>, dim3(c.pairs, p.hkv), kChunkThreads, smem, s, tq, tk, tv, p, c,
+                          PieceWs{}, static_cast<const int*>(flags));
 }
 
 template <int HD, bool BF16, int NORM>
@@ -693,8 +697,8 @@ cudaError_t weights_t(const AttnParams& p, const ChunkPlan& c, float* kw, int64_
   constexpr int smem = WeightLayout<HD>::TOTAL;
   cudaError_t e = allow_smem<chunk_weights_kernel<HD, BF16, NORM>>(smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3((p.len_k + kTileKeys - 1) / kTileKeys, p.hkv, p.batch), kWeightThreads, smem, s>>>(tq, tk, p, c, kw, ldw);
-  return cudaGetLastError();
+  return launch_dependent(kernel, dim3((p.len_k + kTileKeys - 1) / kTileKeys, p.hkv, p.batch), kWeightThreads, smem, s, tq, tk,
+                          p, c, kw, ldw);
 }
 
 // fn<HD, BF16, NORM>(args...) for the request's types.

@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     fence_barrier_init();
   }
   if (warp == 5) tmem_alloc(&bars->tmem, 128);
+  wait_for_predecessor();
   Walk walk(p, c.tpb);
   tc_fence_before();
   __syncthreads();
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 template <int NC>
 __global__ void __launch_bounds__(256) few_weights_kernel(const AttnParams p, const ChunkPlan c, const float* scores,
                                                           float* kw, int64_t ldw) {
+  allow_dependents();
   wait_for_predecessor();
   __shared__ float consts[NC];
   const int b = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
@@ -441,11 +443,11 @@ cudaError_t run(const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw,
   constexpr int smem = FewLayout<HD, NC>::TOTAL;
   cudaError_t e = allow_smem<few_kernel<HD, BF16, NC>>(smem);
   if (e != cudaSuccess) return e;
-  few_kernel<HD, BF16, NC><<<ctas, kFewThreads, smem, s>>>(tq, tk, tv, p, c, ws, scores);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  e = launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, s, p, ws, c.group);
+  e = launch_dependent(few_kernel<HD, BF16, NC>, dim3(ctas), kFewThreads, smem, s, tq, tk, tv, p, c, ws, scores);
+  if (e != cudaSuccess) return e;
+  e = launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, 0, s, p, ws, c.group);
   if (e != cudaSuccess || kw == nullptr) return e;
-  return launch_dependent(few_weights_kernel<NC>, dim3((p.len_k + 255) / 256, p.hkv, p.batch), 256, s, p, c,
+  return launch_dependent(few_weights_kernel<NC>, dim3((p.len_k + 255) / 256, p.hkv, p.batch), 256, 0, s, p, c,
                           static_cast<const float*>(scores), kw, ldw);
 }
 

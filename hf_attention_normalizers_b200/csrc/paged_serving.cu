@@ -18,6 +18,8 @@ namespace {
 template <typename U>
 __global__ void __launch_bounds__(256) append_kernel(AttnParams p, const U* k, const U* v, U* kc, U* vc,
                                                      int units, float* kw, int64_t ldw) {
+  tc::allow_dependents();
+  tc::wait_for_predecessor();
   const int b = blockIdx.y;
   const Geometry g = geometry(p, b);
   const int64_t row_units = (int64_t)p.hkv * units, n = g.q_len * row_units;
@@ -81,6 +83,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(AttnParams p,
                                                                    int recent, int page_shift, int* kept, int* new_lens,
                                                                    int cache) {
   tc::allow_dependents();
+  tc::wait_for_predecessor();
   extern __shared__ uint32_t img[];  // [cache] images of the weights
   __shared__ int hist[kBins];
   __shared__ int wsum[2][kSelWarps];
@@ -231,6 +234,7 @@ template <typename U>
 __global__ void __launch_bounds__(kMoveThreads, 4) evict_move_kernel(AttnParams p, U* kc, U* vc, float* kw, int64_t ldw,
                                                                   int units, int slice, int slices, int budget,
                                                                   int page_shift, const int* kept) {
+  tc::allow_dependents();
   tc::wait_for_predecessor();
   const int h = blockIdx.y, b = blockIdx.z;
   const int L = seq_len_k(p, b);
@@ -304,10 +308,9 @@ cudaError_t append_t(int dtype, const AttnParams& p0, float* kw, int64_t ldw, cu
   const int64_t vecs = (int64_t)p.rows_total * p.hkv * units;
   int64_t gx = (vecs + (int64_t)p.batch * 1024 - 1) / ((int64_t)p.batch * 1024);
   gx = gx < 1 ? 1 : (gx > 4096 ? 4096 : gx);
-  append_kernel<U><<<dim3((unsigned)gx, p.batch), 256, 0, s>>>(
-      p, static_cast<const U*>(p.q), static_cast<const U*>(p.o), static_cast<U*>(const_cast<void*>(p.k)),
-      static_cast<U*>(const_cast<void*>(p.v)), units, kw, ldw);
-  return cudaGetLastError();
+  return launch_dependent(append_kernel<U>, dim3((unsigned)gx, p.batch), 256, 0, s, p, static_cast<const U*>(p.q),
+                          static_cast<const U*>(p.o), static_cast<U*>(const_cast<void*>(p.k)),
+                          static_cast<U*>(const_cast<void*>(p.v)), units, kw, ldw);
 }
 
 template <typename U>
@@ -322,7 +325,7 @@ cudaError_t move_t(int dtype, const AttnParams& p0, float* kw, int64_t ldw, int 
   while (slice % 2 == 0 && slice / 2 >= sector && (int64_t)p.batch * p.hkv * 2 * ((units + slice - 1) / slice) < 2 * sm_count())
     slice /= 2;
   const int slices = (units + slice - 1) / slice;
-  return launch_dependent(evict_move_kernel<U>, dim3(2 * slices + 1, p.hkv, p.batch), kMoveThreads, s, p,
+  return launch_dependent(evict_move_kernel<U>, dim3(2 * slices + 1, p.hkv, p.batch), kMoveThreads, 0, s, p,
                           static_cast<U*>(const_cast<void*>(p.k)), static_cast<U*>(const_cast<void*>(p.v)), kw, ldw, units,
                           slice, slices, budget, page_shift(p), kept);
 }
@@ -346,9 +349,8 @@ cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw
         cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelCache * 4);
     if (e != cudaSuccess) return e;
   }
-  evict_select_kernel<<<dim3(p.hkv, p.batch), kSelThreads, smem, s>>>(p, kw, ldw, budget, recent, page_shift(p), kept, new_lens,
-                                                                                cache);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_dependent(evict_select_kernel, dim3(p.hkv, p.batch), kSelThreads, smem, s, p,
+                                         static_cast<const float*>(kw), ldw, budget, recent, page_shift(p), kept, new_lens, cache);
   if (e != cudaSuccess || p.len_k <= budget) return e;
   const int es = elem_bytes(dtype);
   const bool v = (p.d * es) % 16 == 0 && vec16(p.k, p.k_st, p.k_sh, es) && vec16(p.v, p.v_st, p.v_sh, es);

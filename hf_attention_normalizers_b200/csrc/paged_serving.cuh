@@ -10,6 +10,25 @@
 
 namespace hfan {
 
+// A launch that may be set up while its predecessor on the stream still runs:
+// the kernel calls wait_for_predecessor (tc_ptx.cuh) before it touches memory.
+// Kernels of a few microseconds follow one another here, and their prologues
+// (barriers, TMEM, tensor maps) and launches hide under each other.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // q = new K rows (q_st, q_sh), o = new V rows (o_st, o_sh) -> caches k, v.
 cudaError_t serving_append(int dtype, const AttnParams& p, float* kw, int64_t ldw, cudaStream_t s);
 cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw, int budget, int recent, int* kept,

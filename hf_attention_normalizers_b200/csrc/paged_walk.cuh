@@ -214,19 +214,4 @@ inline PieceWs piece_ws(const AttnParams& p, int ctas, int rows, void* workspace
                  reinterpret_cast<int4*>(base + w.info), rows, ctas};
 }
 
-// A launch that may begin while its predecessor on the stream still runs (it waits inside).
-template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 }  // namespace hfan
