@@ -20,8 +20,10 @@
 // O += P V of j - 1 and S of j + 1 into the buffer that P of j - 1 leaves, so
 // neither side waits for the other's latency.  (One 128-key S buffer a chain,
 // all that fits beside O, left the row warps waiting 1700 of 4600 cycles.)
-// softmax1 keeps a reference m >= 0 (the implicit zero logit) that follows the
-// row maximum lazily: O is rescaled only when the maximum grew by more than 2^8.
+// softmax1 exponentiates against a reference m >= 0 (the implicit zero logit)
+// that need not be the maximum: while the exponentials of a half sum up to at
+// most 2^12, neither P (a 16-bit type) nor O loses anything by it, and no
+// maximum is taken at all.  A row that passes it moves m to its maximum.
 //
 // sparsemax / entmax15 come here with their thresholds known, for the units
 // that the scan (paged_chunk_sparse.cu) could not serve from its buffers.
@@ -42,7 +44,7 @@ using namespace tc;
 
 constexpr int kChunkThreads = 352;
 constexpr int kMaxRing = 8;
-constexpr float kRescale = 8.f;
+constexpr float kHighSum = 4096.f;  // (also keeps P below float16's 65504)
 constexpr int kUnitRows = 2 * kTileRows;
 constexpr int kHalfKeys = kTileKeys / 2;
 
@@ -335,10 +337,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int e = 0; e < 64; ++e) s[e] = e < lim ? s[e] : kNegInf;
           }
           if (NORM == HFAN_SOFTMAX1) {
-            const float top = max_n<64>(s) * zs;
-            if (__any_sync(0xffffffffu, top > m + kRescale)) {
+            float sum;
+            for (bool again = false;; again = true) {
+              const uint64_t zs2 = f2_pack(zs, zs), nm2 = f2_pack(-m, -m);
+              uint64_t l2 = 0;
+#pragma unroll
+              for (int e = 0; e < 64; e += 2) {
+                const uint64_t y = ffma2(f2_pack(s[e], s[e + 1]), zs2, nm2);
+                const float e0 = ex2_ftz(f2_lo(y)), e1 = ex2_ftz(f2_hi(y));
+                l2 = fadd2(l2, f2_pack(e0, e1));
+                pk[e / 2] = pack2<BF16>(e0, e1);
+              }
+              sum = f2_lo(l2) + f2_hi(l2);
+              const bool high = !(sum <= kHighSum);
+              if (again || !__any_sync(0xffffffffu, high)) break;
+              // some row of the warp outgrew its reference: it moves to the
+              // maximum, O and l follow, and the half is exponentiated again
               float alpha = 1.f;
-              if (top > m + kRescale) {
+              if (high) {
+                const float top = fmaxf(max_n<64>(s) * zs, m);
                 alpha = exp2f(m - top);
                 m = top;
                 l *= alpha;
@@ -359,23 +376,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
               }
             }
-          }
-          const uint64_t zs2 = f2_pack(zs, zs), nm2 = f2_pack(-m, -m);
-          uint64_t l2 = 0;
+            if (!ok) break;
+            l += sum;
+          } else {
+            const uint64_t zs2 = f2_pack(zs, zs), nt2 = f2_pack(-m, -m);
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const uint64_t y = ffma2(f2_pack(s[e], s[e + 1]), zs2, nm2);
-            if (NORM == HFAN_SOFTMAX1) {
-              const float e0 = ex2_ftz(f2_lo(y)), e1 = ex2_ftz(f2_hi(y));
-              l2 = fadd2(l2, f2_pack(e0, e1));
-              pk[e / 2] = pack2<BF16>(e0, e1);
-            } else {
+            for (int e = 0; e < 64; e += 2) {
+              const uint64_t y = ffma2(f2_pack(s[e], s[e + 1]), zs2, nt2);
               uint64_t d = f2_pack(fmaxf(f2_lo(y), 0.f), fmaxf(f2_hi(y), 0.f));
               if (NORM == HFAN_ENTMAX15) d = fmul2(d, d);
               pk[e / 2] = pack2<BF16>(f2_lo(d), f2_hi(d));
             }
           }
-          l += f2_lo(l2) + f2_hi(l2);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) pk[e] = 0u;
