@@ -15,6 +15,13 @@
 // sweeps over all keys; a CTA with such a row leaves its P V to the dense
 // kernel (its flag tells it to), which has tau from the statistics.
 //
+// Measured: sparsemax, 4 x 256 tokens on up to 8k keys: 95 us, of a CTA's 138k
+// cycles 101k in the scan, 10k in the threshold, 20k in the gather.  The scan is
+// bound by its row warps: almost every group of 32 columns has a candidate for
+// one of a warp's 32 rows (4.2k cycles a key tile, the products need 1.0k).  A
+// separate pass for the maxima, so that the second one buffers little, took as
+// long as it saved.
+//
 // With few rows a cluster of up to 8 CTAs shares a tile pair, each scanning a
 // part of the keys: the rows' sums are exchanged through distributed shared
 // memory in rank order, so that every rank takes the same steps, and the

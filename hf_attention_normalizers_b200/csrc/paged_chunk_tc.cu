@@ -25,6 +25,13 @@
 // most 2^12, neither P (a 16-bit type) nor O loses anything by it, and no
 // maximum is taken at all.  A row that passes it moves m to its maximum.
 //
+// Measured: 1024 tokens on 32k keys (32 / 8 heads of 128), 0.55 TFLOP: 0.52 ms
+// from a cool start, 0.63 ms in a row, where the 1000 W limit holds the clock at
+// 1.6 GHz; tensor pipe busy 49% of the cycles.  Passing tiles through without
+// any row arithmetic takes 0.43 ms: N = 64 products read Q twice as often, which
+// makes them wait for shared memory (48 cycles instead of 32), the price of the
+// second S buffer.  Loads alone take 0.22 ms.
+//
 // sparsemax / entmax15 come here with their thresholds known, for the units
 // that the scan (paged_chunk_sparse.cu) could not serve from its buffers.
 #include <cuda.h>
@@ -465,6 +472,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 // takes 128 keys of one (sequence, KV head) and walks the row tiles, its two
 // warpgroups alternating between them.  No reference to the maximum is
 // needed: p = 2^(s zs - (m + log2 l)) (softmax1) or (s zs - tau)_+^a.
+// Bound by the exponential unit (16 a cycle and SM): 2 x 512 tokens on 8k keys,
+// 2.7e8 exponentials, 112 us against 63.
 // ---------------------------------------------------------------------------
 struct WeightBars {
   uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2], drain[2];

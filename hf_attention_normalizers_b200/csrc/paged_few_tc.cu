@@ -18,6 +18,11 @@
 // seldom takes that path.  The CTAs walk equal stretches of all key tiles of
 // the batch (paged_walk.cuh).
 //
+// Measured: 8 sequences of 32k keys, one token each, 8 KV heads of 128: 1.07 GB
+// in 178 us, 6.0 TB/s of DRAM reads (0.92 of a copy); 4 sequences of up to 2k
+// keys: 12 us, of which setting up (barriers, TMEM, the walk) takes 2 and the
+// first tile's loads 2.
+//
 // With key weights the raw scores are kept (four bytes a row and key, against
 // the 2 D bytes of the K row), so that the pass over the final statistics reads them
 // instead of K.
