@@ -430,6 +430,30 @@ def test_evict_then_attend():
         _chunk_case(b, norm)
 
 
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 bytes and 2^31 elements, its pages in use at the far end: the same bits as in a small one."""
+    small = Batch([70, 1, 3], [400, 600, 131], seed=50, hkv=8, group=2, interleave=True, stale=0.0)
+    slots = small.key_cache.shape[0]
+    far = (2 ** 31 // (2 * 8 * 128) // 32 + 1) * 32  # the first page whose element offsets pass 2^31
+    both = torch.empty(far + slots, 2, 8, 128, dtype=small.dtype, device="cuda")
+    both[far:, 0], both[far:, 1] = small.d_key, small.d_value
+    weights = torch.zeros(8, far + slots, device="cuda")
+    weights[:, far:] = small.d_weights
+    table = (small.d_table + far // 32).to(torch.int32)
+    new = torch.randn(74, 2, 8, 128, device="cuda").to(small.dtype)
+
+    def run(kc, vc, w, table):
+        serving.paged_append(new[:, 0], new[:, 1], kc, vc, table, small.d_cu, small.d_seq, 32, key_weights=w)
+        outs = [serving.paged_chunk_attention(small.d_query, kc, vc, table, small.d_cu, small.d_seq, 32, norm, key_weights=w,
+                                              max_seqlen_q=n) for norm in NORMS for n in (70, 1)]
+        outs += serving.paged_evict(kc, vc, w, table, small.d_seq, 32, 100, recent=5)
+        return outs + [kc[-slots:], vc[-slots:], w[:, -slots:]]
+
+    for a, b in zip(run(small.d_key, small.d_value, small.d_weights, small.d_table), run(both[:, 0], both[:, 1], weights, table)):
+        assert torch.equal(a, b)
+    assert serving.device_status() == 0
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
