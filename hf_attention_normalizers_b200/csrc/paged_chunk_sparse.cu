@@ -125,7 +125,7 @@ __device__ __noinline__ Scan compact(uint32_t z, uint32_t id, Scan s, int cap, f
     s.gate = raw_gate(t, izs);
   }
   s.n = drop_dead(z, id, s.n, s.thr);
-  if (s.n > cap - 12) s.over = true;  // no room for a chunk of eight
+  if (s.n > cap - 12) s.over = true;  // hardly any room left
   return s;
 }
 
@@ -367,24 +367,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t id0 = t * kTileKeys + cc * 32;
             uint32_t za = zb + sc.n * kZStep, ia = ib + sc.n * kIdStep;
             float gate = sc.over ? kPosInf : sc.gate;
-            // The branches are the warp's, the pushes predicated per lane:
-            // divergent branches around them took several times as long.
+            // Few lanes have a candidate, and those one or two: every lane takes
+            // the quarters of eight it has, one per turn, brings its four scores
+            // to the front by selections and pushes them predicated.  (Divergent
+            // branches took several times as long, 32 predicated pushes twice.)
+            uint32_t mine = 0u;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 8; ++e) mine |= hm[e] > gate ? 1u << e : 0u;
+            while (__any_sync(0xffffffffu, mine != 0u)) {
               // All lanes compact when one has to: they do it in the same time,
               // and their raised bounds keep them from having to one by one.
-              if (e % 2 == 0 && tight) {
+              if (tight) {
                 sc.n = (za - zb) / kZStep;
-                if (__any_sync(0xffffffffu, sc.n > CAP - 8 && !sc.over)) {
+                if (__any_sync(0xffffffffu, sc.n > CAP - 4 && !sc.over)) {
                   sc = compact<NORM>(zb, ib, sc, CAP, izs);
                   za = zb + sc.n * kZStep;
                   ia = ib + sc.n * kIdStep;
                   gate = sc.over ? kPosInf : sc.gate;
                 }
               }
-              if (__any_sync(0xffffffffu, hm[e] > gate)) {
+              const int e = mine != 0u ? __ffs(mine) - 1 : 0;
+              const float lim_e = mine != 0u ? gate : kPosInf;
+              mine &= mine - 1u;
+              const bool b0 = e & 1, b1 = e & 2, b2 = e & 4;
 #pragma unroll
-                for (int j = 4 * e; j < 4 * e + 4; ++j) push_if_above(s[j], gate, s[j] * zs, id0 + j, za, ia, kZStep, kIdStep);
+              for (int k = 0; k < 4; ++k) {
+                const float v0 = b0 ? s[4 + k] : s[k], v1 = b0 ? s[12 + k] : s[8 + k];
+                const float v2 = b0 ? s[20 + k] : s[16 + k], v3 = b0 ? s[28 + k] : s[24 + k];
+                const float x = b2 ? (b1 ? v3 : v2) : (b1 ? v1 : v0);
+                push_if_above(x, lim_e, x * zs, id0 + 4 * e + k, za, ia, kZStep, kIdStep);
               }
             }
             sc.n = (za - zb) / kZStep;
