@@ -15,11 +15,11 @@
 // sweeps over all keys; a CTA with such a row leaves its P V to the dense
 // kernel (its flag tells it to), which has tau from the statistics.
 //
-// Measured: sparsemax, 4 x 256 tokens on up to 8k keys: 95 us, of a CTA's 138k
-// cycles 101k in the scan, 10k in the threshold, 20k in the gather.  The scan is
-// bound by its row warps: almost every group of 32 columns has a candidate for
-// one of a warp's 32 rows (4.2k cycles a key tile, the products need 1.0k).  A
-// separate pass for the maxima, so that the second one buffers little, took as
+// Measured: sparsemax, 4 x up to 256 tokens on up to 8k keys: 85 us, of a CTA's
+// 118k cycles 73k in the scan, 9k in the threshold, 29k in the gather.  The scan
+// is bound by its row warps: three of four groups of 32 columns have a candidate
+// for one of a warp's 32 rows (3.0k cycles a key tile, the products need 1.0k).
+// A separate pass for the maxima, so that the second one buffers little, took as
 // long as it saved.
 //
 // With few rows a cluster of up to 8 CTAs shares a tile pair, each scanning a
@@ -503,16 +503,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* cnt = reinterpret_cast<float*>(smem + L::CNT);
       int* rows = reinterpret_cast<int*>(smem);  // [CAP][256]
       int live = 0;
-#pragma unroll 2
+#pragma unroll 4
       for (int e = 0; e < sc.n; ++e) {
         const float d = lds_f32(zb + e * kZStep) - tau;
-        if (d > 0.f) {
-          const int64_t tok = key_token(p, g, b, kt0 * kTileKeys + (int)lds_u16(ib + e * kIdStep));
-          if (tok >= 0) {
-            sts_f32_if(true, zb + live * kZStep, NORM == HFAN_SPARSEMAX ? d : d * d);
-            rows[live++ * 256 + slot] = (int)tok;
-          }
-        }
+        const uint32_t k = lds_u16(ib + e * kIdStep);
+        const bool in = d > 0.f;
+        sts_f32_if(in, zb + live * kZStep, NORM == HFAN_SPARSEMAX ? d : d * d);
+        sts_u16_if(in, ib + live * kIdStep, k);
+        live += in ? 1 : 0;
+      }
+#pragma unroll 4
+      for (int e = 0; e < live; ++e) {
+        const int64_t tok = key_token(p, g, b, kt0 * kTileKeys + (int)lds_u16(ib + e * kIdStep));
+        sts_f32_if(tok < 0, zb + e * kZStep, 0.f);  // (a page id outside the cache: its V reads as zeros)
+        rows[e * 256 + slot] = max((int)tok, 0);
       }
       cnt[slot] = (float)live;
       __syncwarp();
