@@ -775,7 +775,7 @@ cudaError_t chunk_tc_fwd(int dtype, const AttnParams& p, float* kw, int64_t ldw,
   const ChunkPlan c = plan_of(p);
   if (chunk_few_applies(p, c, kw != nullptr)) return chunk_few_fwd(dtype, p, c, kw, ldw, workspace, s);
   const cudaError_t e = dense_fwd(dtype, p, c, workspace, s);
-  return e != cudaSuccess || kw == nullptr ? e : dense_weights(dtype, p, c, kw, ldw, s);
+  return e != cudaSuccess || kw == nullptr || p.len_k == 0 ? e : dense_weights(dtype, p, c, kw, ldw, s);
 }
 
 }  // namespace hfan

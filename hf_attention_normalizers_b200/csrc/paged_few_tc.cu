@@ -451,7 +451,7 @@ cudaError_t run(const AttnParams& p, const ChunkPlan& c, float* kw, int64_t ldw,
   e = launch_dependent(few_kernel<HD, BF16, NC>, dim3(ctas), kFewThreads, smem, s, tq, tk, tv, p, c, ws, scores);
   if (e != cudaSuccess) return e;
   e = launch_dependent(combine_pieces_kernel<HD, T>, dim3(p.rows_total * p.hkv), 128, 0, s, p, ws, c.group);
-  if (e != cudaSuccess || kw == nullptr) return e;
+  if (e != cudaSuccess || kw == nullptr || p.len_k == 0) return e;
   return launch_dependent(few_weights_kernel<NC>, dim3((p.len_k + 255) / 256, p.hkv, p.batch), 256, 0, s, p, c,
                           static_cast<const float*>(scores), kw, ldw);
 }

@@ -52,10 +52,11 @@ class Walk {
     }
     quota = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 2);
     at_ = (int)blockIdx.x * quota;
-    end_ = min(at_ + quota, total);
-    if (at_ >= end_) return;
+    const int end = min(at_ + quota, total);
+    end_ = at_;
+    if (at_ >= end) return;
     int before = 0;
-    for (int base = 0;; base += 32) {
+    for (int base = 0; base < p.batch; base += 32) {
       const int w = base == 0 ? w0 : (base + lane < p.batch ? sequence_tiles(base + lane) * p.hkv : 0);
       int inc = w;
 #pragma unroll
@@ -67,18 +68,19 @@ class Walk {
       if (hit) {
         const int l = __ffs(hit) - 1;
         enter(base + l);
-        int off = at_ - before - __shfl_sync(0xffffffffu, inc - w, l);
+        int off = max(at_ - before - __shfl_sync(0xffffffffu, inc - w, l), 0);
         const int one = __shfl_sync(0xffffffffu, w, l) / p.hkv;
-        u.kvh = off / one;
+        u.kvh = min(off / one, p.hkv - 1);
         off -= u.kvh * one;
         group_ = 0;
         load_group();
-        while (off >= u.tiles) {
+        while (off >= u.tiles && (group_ + 1) * per_ < u.g.q_len) {
           off -= u.tiles;
           ++group_;
           load_group();
         }
         u0_ = at_ - off;
+        end_ = end;
         break;
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
@@ -96,8 +98,8 @@ class Walk {
         if (++u.kvh == p_.hkv) {
           u.kvh = 0;
           int b = u.b, s;
-          do ++b;
-          while (chunk_tokens(p_, b, &s) == 0);  // (the line has tiles left, so some sequence follows)
+          do ++b;  // (the line has tiles left, so some sequence follows)
+          while (b + 1 < p_.batch && chunk_tokens(p_, b, &s) == 0);
           enter(b);
         }
       }

@@ -430,6 +430,31 @@ def test_evict_then_attend():
         _chunk_case(b, norm)
 
 
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("new", [[2], [50]])
+def test_no_keys_at_all(norm, new):
+    b = Batch(new, [0], seed=51)
+    for kw in (dict(), dict(max_seqlen_k=0)):
+        w = b.weights.cuda()
+        assert (b.chunk(norm, key_weights=w, **kw) == 0).all() and torch.equal(w.cpu(), b.weights)
+    assert serving.device_status() == 0
+
+
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("new", [[1, 2], [60, 70]])
+def test_bad_offsets_stay_inside_the_packed_rows(norm, new):
+    """Offsets past the packed rows, and rows that belong to no sequence: recorded, and nothing outside is touched."""
+    b = Batch(new, [200, 300], seed=52)
+    serving.device_status()
+    b.d_cu = torch.tensor([-3, new[0], 10 ** 6], dtype=torch.int32, device="cuda")
+    b.chunk(norm, key_weights=b.d_weights)
+    assert serving.device_status() == 3
+    b.d_cu = torch.tensor([0, new[0], new[0]], dtype=torch.int32, device="cuda")
+    out, want = b.chunk(norm), b.expected(norm)
+    _check(out[:new[0]], want[0][:new[0]], want[1][:new[0]], norm)
+    assert serving.device_status() == 0
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^32 bytes and 2^31 elements, its pages in use at the far end: the same bits as in a small one."""
     small = Batch([70, 1, 3], [400, 600, 131], seed=50, hkv=8, group=2, interleave=True, stale=0.0)
