@@ -594,14 +594,18 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
     const int key = k0 + r;
     float total = 0.f;
     bool ok = true;
+    // statistics of this thread's row of tile t_lo + u, fetched a tile ahead
+    const int rt = r / c.group, rh = kvh * c.group + r - rt * c.group;
+    auto fetch = [&](int u) -> float2 {
+      if (u >= nt || r >= rows_of(t_lo + u)) return make_float2(0.f, 1.f);
+      const int64_t si = stat_index(p, g, rh, (t_lo + u) * c.tpb + rt);
+      return make_float2(p.stats[si], NORM == HFAN_SOFTMAX1 ? p.stats[(int64_t)p.hq * p.rows_total + si] : 1.f);
+    };
+    float2 ahead = fetch(w);
     for (int u = w; u < nt; u += 2) {
       const int t = t_lo + u, nrows = rows_of(t);
-      float cst = 0.f;
-      if (r < nrows) {
-        const int64_t si = stat_index(p, g, kvh * c.group + r % c.group, t * c.tpb + r / c.group);
-        const float s0 = p.stats[si];
-        cst = NORM == HFAN_SOFTMAX1 ? -(s0 + log2f(p.stats[(int64_t)p.hq * p.rows_total + si])) : -s0;
-      }
+      const float cst = NORM == HFAN_SOFTMAX1 ? -(ahead.x + log2f(ahead.y)) : -ahead.x;
+      ahead = fetch(u + 2);
       named_bar_sync(1 + w, 128);  // the previous tile's constants have been read
       consts[r] = cst;
       named_bar_sync(1 + w, 128);
