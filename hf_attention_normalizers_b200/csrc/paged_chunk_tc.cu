@@ -26,7 +26,7 @@
 // maximum is taken at all.  A row that passes it moves m to its maximum.
 //
 // Measured: 1024 tokens on 32k keys (32 / 8 heads of 128), 0.55 TFLOP: 0.52 ms
-// from a cool start, 0.63 ms in a row, where the 1000 W limit holds the clock at
+// from a cool start, 0.64 ms in a row, where the 1000 W limit holds the clock at
 // 1.6 GHz; tensor pipe busy 49% of the cycles.  Passing tiles through without
 // any row arithmetic takes 0.43 ms: N = 64 products read Q twice as often, which
 // makes them wait for shared memory (48 cycles instead of 32), the price of the

@@ -138,9 +138,6 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
 __device__ __forceinline__ void sts_u16(uint32_t addr, uint16_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
-__device__ __forceinline__ void sts_b32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
 // ---------------------------------------------------------------- cluster
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -172,11 +169,6 @@ __device__ __forceinline__ float4 peer_ld4(const float4* p, uint32_t rank) {
 __device__ __forceinline__ float peer_ldf(const float* p, uint32_t rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_smem(p, rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t peer_ldu16(const uint16_t* p, uint32_t rank) {
-  uint16_t v;
-  asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(peer_smem(p, rank)) : "memory");
   return v;
 }
 // mbar_wait that also acquires what other CTAs of the cluster wrote before they arrived.
