@@ -298,7 +298,7 @@ int fill_chunk(const hfan_chunk_desc* desc, AttnParams& p) {
   p.hq = desc->heads_q;
   p.hkv = desc->heads_kv;
   p.d = desc->head_dim;
-  p.len_q = desc->max_len_q;
+  p.len_q = desc->max_len_q > 0 ? desc->max_len_q : 1;  // (sizes tiles and grids; longer chunks are served all the same)
   p.len_k = desc->max_len_k;
   p.rows_total = desc->total_q;
   p.cu_q = desc->cu_seqlens_q;
@@ -505,7 +505,7 @@ int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor
   int rc = fill_chunk_rows(desc, p);
   if (rc != HFAN_OK) return rc;
   if ((rc = check_weights(desc, key_weights, ld_weights)) != HFAN_OK) return rc;
-  if (desc->total_q == 0 || desc->max_len_q == 0) return HFAN_OK;
+  if (desc->total_q == 0) return HFAN_OK;
   if (stats == nullptr) return fail(HFAN_ERR_INVALID, "stats buffer is required");
   p.stats = stats;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -518,7 +518,7 @@ int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor
       return fail(HFAN_ERR_INVALID, "paged chunk: workspace must be 256-byte aligned");
     e = chunk_tc_fwd(desc->dtype, p, key_weights, ld_weights, workspace, s);
   } else {
-    e = simt_attention_fwd(desc->dtype, p, desc->max_len_q, s);
+    e = simt_attention_fwd(desc->dtype, p, p.len_q, s);
     if (e == cudaSuccess && key_weights != nullptr && desc->max_len_k > 0)
       e = serving_key_weights(desc->dtype, p, key_weights, ld_weights, s);
   }

@@ -64,128 +64,129 @@ __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Geometry g = geometry(p, b);
-  const int q0 = blockIdx.x * kRows;
-  if (q0 >= g.q_len) return;
-  const int row = q0 + warp;
-  const bool active = row < g.q_len;
   const int kvh = h / (p.hq / p.hkv);
   const T* qp = static_cast<const T*>(p.q);
   const T* kp = static_cast<const T*>(p.k);
   const T* vp = static_cast<const T*>(p.v);
-
-  for (int d = lane; d < D; d += 32)
-    Qs[warp * D + d] = active ? to_f32<T>(qp[qrow_off(p, g, b, h, row, p.q_sb, p.q_sh, p.q_st) + d]) : 0.f;
-
-  const int last_row = min(q0 + kRows - 1, g.q_len - 1);
-  int k_hi = g.k_len;
-  if (p.causal) k_hi = min(k_hi, last_row + g.shift + 1);
-  int k_lo = 0;
-  if (p.window_left > 0) k_lo = max(0, q0 + g.shift - p.window_left + 1);
-  k_lo = (k_lo / kTile) * kTile;
   const float zs = zscale_of<NORM>(p.scale);
+  // (one turn of the loop, unless the grid was sized by a bound that the sequence passes)
+  for (int q0 = blockIdx.x * kRows; q0 < g.q_len; q0 += gridDim.x * kRows) {
+    const int row = q0 + warp;
+    const bool active = row < g.q_len;
 
-  auto score = [&](int kb) -> float {
-    int j = kb + lane;
-    float s = dot_row(Qs + warp * D, Ks + lane * Dp, D);
-    return (active && key_visible(row, j, g, p.causal, p.window_left)) ? s * zs : kNegInf;
-  };
+    for (int d = lane; d < D; d += 32)
+      Qs[warp * D + d] = active ? to_f32<T>(qp[qrow_off(p, g, b, h, row, p.q_sb, p.q_sh, p.q_st) + d]) : 0.f;
 
-  float acc[kMaxDimRegs];
+    const int last_row = min(q0 + kRows - 1, g.q_len - 1);
+    int k_hi = g.k_len;
+    if (p.causal) k_hi = min(k_hi, last_row + g.shift + 1);
+    int k_lo = 0;
+    if (p.window_left > 0) k_lo = max(0, q0 + g.shift - p.window_left + 1);
+    k_lo = (k_lo / kTile) * kTile;
+
+    auto score = [&](int kb) -> float {
+      int j = kb + lane;
+      float s = dot_row(Qs + warp * D, Ks + lane * Dp, D);
+      return (active && key_visible(row, j, g, p.causal, p.window_left)) ? s * zs : kNegInf;
+    };
+
+    float acc[kMaxDimRegs];
 #pragma unroll
-  for (int i = 0; i < kMaxDimRegs; ++i) acc[i] = 0.f;
-  auto accumulate_pv = [&](float pj) {
-    for (int jj = 0; jj < kTile; ++jj) {
-      float pr = __shfl_sync(0xffffffffu, pj, jj);
-      if (pr != 0.f) {
+    for (int i = 0; i < kMaxDimRegs; ++i) acc[i] = 0.f;
+    auto accumulate_pv = [&](float pj) {
+      for (int jj = 0; jj < kTile; ++jj) {
+        float pr = __shfl_sync(0xffffffffu, pj, jj);
+        if (pr != 0.f) {
 #pragma unroll
-        for (int i = 0; i < kMaxDimRegs; ++i) {
-          int d = lane + 32 * i;
-          if (d < D) acc[i] = fmaf(pr, Vs[jj * Dp + d], acc[i]);
+          for (int i = 0; i < kMaxDimRegs; ++i) {
+            int d = lane + 32 * i;
+            if (d < D) acc[i] = fmaf(pr, Vs[jj * Dp + d], acc[i]);
+          }
         }
       }
-    }
-  };
+    };
 
-  float stat0, stat1;
-  if (NORM == HFAN_SOFTMAX1) {
-    // Online max / denominator seeded with the implicit zero logit (m = 0,
-    // l = 1), as kernels/softmax1_hopper.py:80-83; log2 units.
-    float m = 0.f, l = 1.f;
-    for (int kb = k_lo; kb < k_hi; kb += kTile) {
-      __syncthreads();
-      load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
-      load_key_tile<T>(p, g, b, kvh, kb, k_hi, vp, p.v_sb, p.v_sh, p.v_st, Vs, Dp);
-      __syncthreads();
-      float z = score(kb);
-      float m_new = fmaxf(m, warp_max(z));
-      float alpha = exp2f(m - m_new);
-      float pj = (z == kNegInf) ? 0.f : exp2f(z - m_new);
-      l = l * alpha + warp_sum(pj);
+    float stat0, stat1;
+    if (NORM == HFAN_SOFTMAX1) {
+      // Online max / denominator seeded with the implicit zero logit (m = 0,
+      // l = 1), as kernels/softmax1_hopper.py:80-83; log2 units.
+      float m = 0.f, l = 1.f;
+      for (int kb = k_lo; kb < k_hi; kb += kTile) {
+        __syncthreads();
+        load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
+        load_key_tile<T>(p, g, b, kvh, kb, k_hi, vp, p.v_sb, p.v_sh, p.v_st, Vs, Dp);
+        __syncthreads();
+        float z = score(kb);
+        float m_new = fmaxf(m, warp_max(z));
+        float alpha = exp2f(m - m_new);
+        float pj = (z == kNegInf) ? 0.f : exp2f(z - m_new);
+        l = l * alpha + warp_sum(pj);
 #pragma unroll
-      for (int i = 0; i < kMaxDimRegs; ++i) acc[i] *= alpha;
-      accumulate_pv(pj);
-      m = m_new;
-    }
-    float inv = 1.f / l;
+        for (int i = 0; i < kMaxDimRegs; ++i) acc[i] *= alpha;
+        accumulate_pv(pj);
+        m = m_new;
+      }
+      float inv = 1.f / l;
 #pragma unroll
-    for (int i = 0; i < kMaxDimRegs; ++i) acc[i] *= inv;
-    stat0 = m;
-    stat1 = l;
-  } else {
-    // Pass 1: row max.
-    float zmax = kNegInf;
-    for (int kb = k_lo; kb < k_hi; kb += kTile) {
-      __syncthreads();
-      load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
-      __syncthreads();
-      zmax = fmaxf(zmax, warp_max(score(kb)));
-    }
-    const bool empty = !(zmax > kNegInf);
-    bool done = empty || !active;
-    float t = zmax - 1.f, tau = kPosInf;
-    // Exact threshold: bracket sweeps until the candidate set is the support.
-    for (int it = 0; it < 64; ++it) {
-      if (!__syncthreads_or(!done)) break;
-      TauStats st{0.f, 0.f, 0.f, kPosInf};
+      for (int i = 0; i < kMaxDimRegs; ++i) acc[i] *= inv;
+      stat0 = m;
+      stat1 = l;
+    } else {
+      // Pass 1: row max.
+      float zmax = kNegInf;
       for (int kb = k_lo; kb < k_hi; kb += kTile) {
         __syncthreads();
         load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
         __syncthreads();
-        float z = score(kb);
-        if (!done) tau_accumulate(st, z, t);
+        zmax = fmaxf(zmax, warp_max(score(kb)));
       }
-      st.cnt = warp_sum(st.cnt);
-      st.s1 = warp_sum(st.s1);
-      st.s2 = warp_sum(st.s2);
-      st.zmin = warp_min(st.zmin);
-      if (!done) done = tau_step(NORM, st, &t, &tau);
+      const bool empty = !(zmax > kNegInf);
+      bool done = empty || !active;
+      float t = zmax - 1.f, tau = kPosInf;
+      // Exact threshold: bracket sweeps until the candidate set is the support.
+      for (int it = 0; it < 64; ++it) {
+        if (!__syncthreads_or(!done)) break;
+        TauStats st{0.f, 0.f, 0.f, kPosInf};
+        for (int kb = k_lo; kb < k_hi; kb += kTile) {
+          __syncthreads();
+          load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
+          __syncthreads();
+          float z = score(kb);
+          if (!done) tau_accumulate(st, z, t);
+        }
+        st.cnt = warp_sum(st.cnt);
+        st.s1 = warp_sum(st.s1);
+        st.s2 = warp_sum(st.s2);
+        st.zmin = warp_min(st.zmin);
+        if (!done) done = tau_step(NORM, st, &t, &tau);
+      }
+      float support = 0.f;
+      for (int kb = k_lo; kb < k_hi; kb += kTile) {
+        __syncthreads();
+        load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
+        load_key_tile<T>(p, g, b, kvh, kb, k_hi, vp, p.v_sb, p.v_sh, p.v_st, Vs, Dp);
+        __syncthreads();
+        float z = score(kb);
+        float pj = (active && !empty) ? sparse_prob(NORM, z, tau) : 0.f;
+        support += warp_sum(pj > 0.f ? 1.f : 0.f);
+        accumulate_pv(pj);
+      }
+      stat0 = empty ? kPosInf : tau;
+      stat1 = support;
     }
-    float support = 0.f;
-    for (int kb = k_lo; kb < k_hi; kb += kTile) {
-      __syncthreads();
-      load_key_tile<T>(p, g, b, kvh, kb, k_hi, kp, p.k_sb, p.k_sh, p.k_st, Ks, Dp);
-      load_key_tile<T>(p, g, b, kvh, kb, k_hi, vp, p.v_sb, p.v_sh, p.v_st, Vs, Dp);
-      __syncthreads();
-      float z = score(kb);
-      float pj = (active && !empty) ? sparse_prob(NORM, z, tau) : 0.f;
-      support += warp_sum(pj > 0.f ? 1.f : 0.f);
-      accumulate_pv(pj);
-    }
-    stat0 = empty ? kPosInf : tau;
-    stat1 = support;
-  }
 
-  if (active) {
-    T* op = static_cast<T*>(p.o) + qrow_off(p, g, b, h, row, p.o_sb, p.o_sh, p.o_st);
+    if (active) {
+      T* op = static_cast<T*>(p.o) + qrow_off(p, g, b, h, row, p.o_sb, p.o_sh, p.o_st);
 #pragma unroll
-    for (int i = 0; i < kMaxDimRegs; ++i) {
-      int d = lane + 32 * i;
-      if (d < D) op[d] = from_f32<T>(acc[i]);
-    }
-    if (lane == 0) {
-      int64_t si = stat_index(p, g, h, row);
-      p.stats[si] = stat0;
-      p.stats[(int64_t)p.hq * p.rows_total + si] = stat1;
+      for (int i = 0; i < kMaxDimRegs; ++i) {
+        int d = lane + 32 * i;
+        if (d < D) op[d] = from_f32<T>(acc[i]);
+      }
+      if (lane == 0) {
+        int64_t si = stat_index(p, g, h, row);
+        p.stats[si] = stat0;
+        p.stats[(int64_t)p.hq * p.rows_total + si] = stat1;
+      }
     }
   }
 }

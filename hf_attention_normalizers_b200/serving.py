@@ -24,9 +24,11 @@ Shapes (T new tokens of B sequences packed one after the other):
 Inference only: nothing here has a gradient (``paged.paged_attention`` has).
 No call waits for the GPU; lengths, offsets and page ids are checked on the
 device, where a bad one is clamped or skipped and recorded in the status word
-that ``device_status`` reads.  ``max_seqlen_q`` / ``max_seqlen_k`` are upper
-bounds known to the host; without them the packed length and the block table's
-capacity are taken, which costs idle thread blocks.
+that ``device_status`` reads.  ``max_seqlen_q`` / ``max_seqlen_k`` are what the host
+knows of the longest; without them the packed length and the block table's
+capacity are taken, which costs idle thread blocks.  More new tokens than
+``max_seqlen_q`` only cost time; keys past ``max_seqlen_k`` are cut off, as a
+bad length.
 """
 
 from __future__ import annotations

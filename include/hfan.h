@@ -252,10 +252,11 @@ typedef struct hfan_chunk_desc {
   int32_t heads_kv;
   int32_t head_dim;
   int32_t total_q;              /* packed new tokens                                     */
-  int32_t max_len_q;            /* upper bound of one sequence's new tokens              */
+  int32_t max_len_q;            /* the most new tokens of one sequence: sizes tiles and
+                                 * grids; longer chunks are served all the same          */
   int32_t page_size;
   int32_t max_blocks;           /* block_table row stride (columns)                      */
-  int32_t max_len_k;            /* upper bound of seq_lens                               */
+  int32_t max_len_k;            /* upper bound of seq_lens: longer ones are clamped      */
   int64_t num_cache_tokens;
   const int32_t* block_table;   /* [batch, max_blocks] physical page ids                 */
   const int32_t* cu_seqlens_q;  /* [batch + 1]                                           */

@@ -318,6 +318,24 @@ def test_bad_page_and_length_are_recorded():
         assert serving.device_status() == 3
 
 
+def _stale_results(b):
+    """Leave NaN in the allocator's blocks that the next call's output and statistics will take."""
+    junk = [torch.full_like(b.d_query, float("nan")) for _ in range(3)]
+    junk += [torch.full((2, b.query.shape[1], b.query.shape[0]), float("nan"), device="cuda") for _ in range(3)]
+    del junk
+
+
+@pytest.mark.parametrize("hint", [0, 2])
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("kw", [dict(), dict(dtype=torch.float32), dict(dim=40), dict(page=5), dict(group=48, hkv=1),
+                                dict(group=160, hkv=1, dim=64)])
+def test_low_hint_of_the_longest_chunk(kw, norm, hint):
+    """Rows past the hint are computed all the same, by every kernel."""
+    b = Batch([40, 3], [300, 130], seed=53, gain=2.0, **kw)
+    _stale_results(b)
+    _chunk_case(b, norm, max_seqlen_q=hint)
+
+
 # ---------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------
