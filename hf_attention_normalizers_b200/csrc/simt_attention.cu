@@ -54,7 +54,10 @@ __device__ __forceinline__ float dot_row(const float* a, const float* bvec, int 
 // --------------------------------------------------------------------------
 // Forward
 // --------------------------------------------------------------------------
-template <typename T, int NORM>
+// RAGGED: a chunk over a paged cache, whose lengths the host does not know for
+// certain; a block then walks the rows past the grid as well.  (An instance of
+// its own: the loop around the body cost the other callers spilled registers.)
+template <typename T, int NORM, bool RAGGED>
 __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
   extern __shared__ float smem[];
   const int D = p.d, Dp = D + 1;
@@ -69,7 +72,6 @@ __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
   const T* kp = static_cast<const T*>(p.k);
   const T* vp = static_cast<const T*>(p.v);
   const float zs = zscale_of<NORM>(p.scale);
-  // (one turn of the loop, unless the grid was sized by a bound that the sequence passes)
   for (int q0 = blockIdx.x * kRows; q0 < g.q_len; q0 += gridDim.x * kRows) {
     const int row = q0 + warp;
     const bool active = row < g.q_len;
@@ -188,6 +190,7 @@ __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
         p.stats[(int64_t)p.hq * p.rows_total + si] = stat1;
       }
     }
+    if (!RAGGED) break;
   }
 }
 
@@ -482,10 +485,17 @@ template <typename T>
 static cudaError_t fwd_t(const AttnParams& p, int max_q, cudaStream_t s) {
   dim3 grid((max_q + kRows - 1) / kRows, p.hq, p.batch);
   size_t sm = simt_fwd_smem(p.d);
+  if (p.paged && p.cu_q != nullptr) {
+    switch (p.norm) {
+      case HFAN_SOFTMAX1: return launch(simt_fwd_kernel<T, HFAN_SOFTMAX1, true>, grid, sm, s, p);
+      case HFAN_SPARSEMAX: return launch(simt_fwd_kernel<T, HFAN_SPARSEMAX, true>, grid, sm, s, p);
+      default: return launch(simt_fwd_kernel<T, HFAN_ENTMAX15, true>, grid, sm, s, p);
+    }
+  }
   switch (p.norm) {
-    case HFAN_SOFTMAX1: return launch(simt_fwd_kernel<T, HFAN_SOFTMAX1>, grid, sm, s, p);
-    case HFAN_SPARSEMAX: return launch(simt_fwd_kernel<T, HFAN_SPARSEMAX>, grid, sm, s, p);
-    default: return launch(simt_fwd_kernel<T, HFAN_ENTMAX15>, grid, sm, s, p);
+    case HFAN_SOFTMAX1: return launch(simt_fwd_kernel<T, HFAN_SOFTMAX1, false>, grid, sm, s, p);
+    case HFAN_SPARSEMAX: return launch(simt_fwd_kernel<T, HFAN_SPARSEMAX, false>, grid, sm, s, p);
+    default: return launch(simt_fwd_kernel<T, HFAN_ENTMAX15, false>, grid, sm, s, p);
   }
 }
 
