@@ -345,13 +345,11 @@ cudaError_t serving_evict(int dtype, const AttnParams& p, float* kw, int64_t ldw
                           int* new_lens, cudaStream_t s) {
   const int cache = p.len_k < kSelCache ? p.len_k : kSelCache;
   const size_t smem = (size_t)cache * 4;
-  if (smem > 40 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelCache * 4);
-    if (e != cudaSuccess) return e;
-  }
-  const cudaError_t e = launch_dependent(evict_select_kernel, dim3(p.hkv, p.batch), kSelThreads, smem, s, p,
-                                         static_cast<const float*>(kw), ldw, budget, recent, page_shift(p), kept, new_lens, cache);
+  // (asked for at every length: what a launch may have by default holds the static arrays too)
+  cudaError_t e = allow_smem<evict_select_kernel>(kSelCache * 4);
+  if (e != cudaSuccess) return e;
+  e = launch_dependent(evict_select_kernel, dim3(p.hkv, p.batch), kSelThreads, smem, s, p, static_cast<const float*>(kw), ldw,
+                       budget, recent, page_shift(p), kept, new_lens, cache);
   if (e != cudaSuccess || p.len_k <= budget) return e;
   const int es = elem_bytes(dtype);
   const bool v = (p.d * es) % 16 == 0 && vec16(p.k, p.k_st, p.k_sh, es) && vec16(p.v, p.v_st, p.v_sh, es);

@@ -430,6 +430,23 @@ def test_evict_ties_zeros_infinities_and_nan():
     _evict_case(b, 450, 9)
 
 
+def _evict_around_the_default_shared_memory():
+    for keys in (10172, 10173, 10240, 10241):
+        _evict_case(Batch([1], [keys], seed=54, hkv=1, dim=64), 300, 7, max_seqlen_k=keys)
+
+
+def test_evict_around_the_default_shared_memory():
+    """The selection's static and dynamic shared memory pass what a launch may have without asking.
+
+    In a process of its own: once a kernel was given more, it keeps it."""
+    import multiprocessing
+
+    child = multiprocessing.get_context("spawn").Process(target=_evict_around_the_default_shared_memory)
+    child.start()
+    child.join(300)
+    assert child.exitcode == 0
+
+
 def test_evict_longer_than_shared_memory_holds():
     """Past 45056 candidates the selection reads the rest of the weights again in every pass."""
     _evict_case(Batch([1], [50000], seed=33, hkv=1, dim=64, page=64), 1200, 33)
