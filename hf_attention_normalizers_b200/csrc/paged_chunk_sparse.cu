@@ -150,6 +150,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tm_k);
   }
   wait_for_predecessor();
+  const UnownedRows rest(p);
+  for (int x = blockIdx.x; x < rest.count; x += gridDim.x)
+    store_empty_rows<T, uint4>(p, rest.at(x), blockIdx.y * c.group, c.group);
   int b, pair;
   const int unit = blockIdx.x / ranks;
   if (!find_group(p, 2 * c.tpb, unit, &b, &pair)) return;  // the whole cluster alike

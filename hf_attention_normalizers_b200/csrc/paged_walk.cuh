@@ -143,13 +143,18 @@ class Walk {
 };
 
 // Joins the pieces of split units: one block per (token, KV head) and its G rows.
+// Tokens that no sequence owns get theirs here.
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) combine_pieces_kernel(const AttnParams p, const PieceWs ws, int group) {
   tc::allow_dependents();
   tc::wait_for_predecessor();  // (set up while the pieces are still being computed)
   const int tok = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
   const int4 f = ws.info[blockIdx.x];
-  // (a token that no sequence owns has no info: kept inside the workspace)
+  if (UnownedRows(p).holds(tok)) {
+    store_empty_rows<T, uint2>(p, tok, kvh * group, group);
+    return;
+  }
+  // (under offsets that decrease a token may have no info: kept inside the workspace)
   const int quota = max(f.w, 1), first = min(max(f.x / quota, 0), ws.ctas - 1);
   const int last = min(max((f.x + f.y - 1) / quota, first), ws.ctas - 1);
   if (last == first) return;

@@ -177,6 +177,34 @@ __device__ __forceinline__ int64_t key_off(const AttnParams& p, int b, int kvh, 
   return bo + (int64_t)kvh * sh + tok * st;
 }
 
+// Packed rows of a ragged chunk that no sequence owns (a padded batch): those
+// before the first offset and past the last one, `count` of them.
+struct UnownedRows {
+  int first, last, count;
+  __device__ __forceinline__ explicit UnownedRows(const AttnParams& p) {
+    first = min(max(p.cu_q[0], 0), p.rows_total);
+    last = min(max(p.cu_q[p.batch], first), p.rows_total);
+    count = first + p.rows_total - last;
+  }
+  __device__ __forceinline__ bool holds(int tok) const { return tok < first || tok >= last; }
+  __device__ __forceinline__ int at(int x) const { return x < first ? x : x - first + last; }
+};
+
+// Output and statistics of `heads` query heads of a token that sees no key.
+// Whole-block call; a row of the output is stored in vectors U.
+template <typename T, typename U>
+__device__ __forceinline__ void store_empty_rows(const AttnParams& p, int tok, int h0, int heads) {
+  const int units = p.d * (int)sizeof(T) / (int)sizeof(U);
+  for (int x = threadIdx.x; x < heads * units; x += blockDim.x) {
+    const int h = h0 + x / units, c = x % units;
+    reinterpret_cast<U*>(static_cast<T*>(p.o) + (int64_t)tok * p.o_st + (int64_t)h * p.o_sh)[c] = U();
+    if (c == 0) {
+      p.stats[(int64_t)h * p.rows_total + tok] = p.norm == HFAN_SOFTMAX1 ? 0.f : __int_as_float(0x7f800000);
+      p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = p.norm == HFAN_SOFTMAX1 ? 1.f : 0.f;
+    }
+  }
+}
+
 __device__ __forceinline__ int64_t stat_index(const AttnParams& p, const Geometry& g, int h, int i) {
   return (int64_t)h * p.rows_total + g.q_start + i;
 }

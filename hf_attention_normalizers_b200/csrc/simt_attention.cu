@@ -55,8 +55,9 @@ __device__ __forceinline__ float dot_row(const float* a, const float* bvec, int 
 // Forward
 // --------------------------------------------------------------------------
 // RAGGED: a chunk over a paged cache, whose lengths the host does not know for
-// certain; a block then walks the rows past the grid as well.  (An instance of
-// its own: the loop around the body cost the other callers spilled registers.)
+// certain; a block then walks the rows past the grid as well, and those that no
+// sequence owns.  (An instance of its own: the loop around the body cost the
+// other callers spilled registers.)
 template <typename T, int NORM, bool RAGGED>
 __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
   extern __shared__ float smem[];
@@ -72,6 +73,10 @@ __global__ void __launch_bounds__(kRows * 32) simt_fwd_kernel(AttnParams p) {
   const T* kp = static_cast<const T*>(p.k);
   const T* vp = static_cast<const T*>(p.v);
   const float zs = zscale_of<NORM>(p.scale);
+  if (RAGGED && b == 0) {
+    const UnownedRows rest(p);
+    for (int x = blockIdx.x; x < rest.count; x += gridDim.x) store_empty_rows<T, T>(p, rest.at(x), h, 1);
+  }
   for (int q0 = blockIdx.x * kRows; q0 < g.q_len; q0 += gridDim.x * kRows) {
     const int row = q0 + warp;
     const bool active = row < g.q_len;

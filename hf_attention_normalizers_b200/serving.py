@@ -134,7 +134,8 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     """Attention of a ragged chunk of new tokens ``[T, q_heads, dim]`` over the cached context.
 
     The causal mask is aligned to each sequence's end (its new tokens are its
-    last keys); rows that see no key give zeros.  Cache slots past a sequence's
+    last keys); rows that see no key give zeros, and so do the packed rows that
+    no sequence owns (padding before the first offset or past the last).  Cache slots past a sequence's
     length are never used, whatever they hold.  With ``key_weights`` the
     probabilities of every key, summed over the new tokens and the query heads
     of its KV head, are added to its accumulator.

@@ -243,7 +243,8 @@ int hfan_paged_decode_static(const hfan_paged_desc* desc, hfan_tensor q, hfan_te
  * accumulator per KV head and cache slot, ld >= num_cache_tokens.
  * The offsets and lengths stay on the device: out-of-range ones are clamped and
  * recorded in the device status word (see hfan_device_status).  Sequences may
- * bring no token; rows that see no key give a zero row. */
+ * bring no token; rows that see no key give a zero row, and so do packed rows
+ * before cu_seqlens_q[0] and from cu_seqlens_q[batch] on. */
 typedef struct hfan_chunk_desc {
   int32_t dtype;
   int32_t normalizer;

@@ -336,6 +336,26 @@ def test_low_hint_of_the_longest_chunk(kw, norm, hint):
     _chunk_case(b, norm, max_seqlen_q=hint)
 
 
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("kw", [dict(), dict(dtype=torch.float32), dict(dim=64, dtype=torch.float16, group=3)])
+@pytest.mark.parametrize("new,lens", [([1, 2], [200, 300]), ([60, 70], [200, 300]), ([0, 0], [20, 7])])
+def test_rows_of_no_sequence_are_zero(new, lens, kw, norm):
+    """A padded batch: packed rows before the first offset and past the last one."""
+    b = Batch(new, lens, seed=55, gain=2.0, **kw)
+    want, tol, add, add_tol = b.expected(norm)
+    front, back, n = 5, 37, sum(new)
+    query = torch.full((front + n + back, *b.query.shape[1:]), 3.0, dtype=b.dtype, device="cuda")
+    query[front:front + n] = b.d_query
+    b.d_query, b.query, b.d_cu = query, query, b.d_cu + front
+    _stale_results(b)
+    out = b.chunk(norm, key_weights=b.d_weights)
+    assert (out[:front] == 0).all() and (out[front + n:] == 0).all()
+    _check(out[front:front + n], want, tol, norm) if n else None
+    before = b.weights.double().numpy()
+    _check(b.d_weights, before + add, add_tol + 1e-6 * (before + add), f"{norm}/weights")
+    assert serving.device_status() == 0
+
+
 # ---------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------
