@@ -20,10 +20,13 @@
 // O += P V of j - 1 and S of j + 1 into the buffer that P of j - 1 leaves, so
 // neither side waits for the other's latency.  (One 128-key S buffer a chain,
 // all that fits beside O, left the row warps waiting 1700 of 4600 cycles.)
-// softmax1 exponentiates against a reference m >= 0 (the implicit zero logit)
-// that need not be the maximum: while the exponentials of a half sum up to at
-// most 2^12, neither P (a 16-bit type) nor O loses anything by it, and no
-// maximum is taken at all.  A row that passes it moves m to its maximum.
+// softmax1 exponentiates against a reference m that need not be the maximum:
+// while the exponentials of a half sum up to at most 2^12, O loses nothing by
+// it, and no maximum is taken at all.  A row that passes it moves m to its
+// maximum.  m starts at the implicit zero logit in bfloat16, whose exponents
+// reach as far as float32's, so that P loses nothing on the low side either; in
+// float16 it starts 2^8 below the maximum of the piece's first half and moves
+// past a sum of 2^15, see reference16 (paged_walk.cuh).
 //
 // Measured: 1024 tokens on 32k keys (32 / 8 heads of 128), 0.55 TFLOP: 0.52 ms
 // from a cool start, 0.64 ms in a row, where the 1000 W limit holds the clock at
@@ -51,7 +54,8 @@ using namespace tc;
 
 constexpr int kChunkThreads = 352;
 constexpr int kMaxRing = 8;
-constexpr float kHighSum = 4096.f;  // (also keeps P below float16's 65504)
+template <bool BF16>
+constexpr float kHighSum = BF16 ? 4096.f : 32768.f;  // (also keeps P below float16's 65504)
 constexpr int kUnitRows = 2 * kTileRows;
 constexpr int kHalfKeys = kTileKeys / 2;
 
@@ -345,6 +349,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           if (NORM == HFAN_SOFTMAX1) {
             float sum;
+            if (!BF16 && j == 0) m = reference16(max_n<64>(s) * zs);
             for (bool again = false;; again = true) {
               const uint64_t zs2 = f2_pack(zs, zs), nm2 = f2_pack(-m, -m);
               uint64_t l2 = 0;
@@ -356,15 +361,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 pk[e / 2] = pack2<BF16>(e0, e1);
               }
               sum = f2_lo(l2) + f2_hi(l2);
-              const bool high = !(sum <= kHighSum);
+              const bool high = !(sum <= kHighSum<BF16>);
               if (again || !__any_sync(0xffffffffu, high)) break;
               // some row of the warp outgrew its reference: it moves to the
               // maximum, O and l follow, and the half is exponentiated again
               float alpha = 1.f;
               if (high) {
-                const float top = fmaxf(max_n<64>(s) * zs, m);
-                alpha = exp2f(m - top);
-                m = top;
+                const float top = max_n<64>(s) * zs, ref = fmaxf(BF16 ? top : reference16(top), m);
+                alpha = exp2f(m - ref);
+                m = ref;
                 l *= alpha;
               }
               if (j > 0) {
@@ -410,8 +415,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (ok) ok = wait_warp(&bars->pv_done[q], (jj - 2) & 1, abort_flag) && wait_warp(&bars->pv_done[q], (jj - 1) & 1, abort_flag);
       tc_fence_after();
       const int row_in_unit = q * kTileRows + r;
-      if (NORM == HFAN_SOFTMAX1 && pc.whole) l += exp2f(-m);  // the implicit zero logit
-      const float inv = NORM == HFAN_SOFTMAX1 && pc.whole ? 1.f / l : 1.f;
+      const RowEnd end = end_of_row<BF16>(m, l);
+      const float inv = NORM == HFAN_SOFTMAX1 ? end.inv : 1.f;  // (of whole pieces)
       T* dst = static_cast<T*>(p.o) + (int64_t)(u.g.q_start + i) * p.o_st + (int64_t)h * p.o_sh;
       float* part = ws.o + ((int64_t)pc.slot * kUnitRows + row_in_unit) * HD;
 #pragma unroll 1
@@ -445,8 +450,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       warp_arrive(&bars->o_empty[q]);
       if (NORM == HFAN_SOFTMAX1 && row_ok) {
         if (pc.whole) {
-          p.stats[si] = m;
-          p.stats[(int64_t)p.hq * p.rows_total + si] = l;
+          p.stats[si] = end.m;
+          p.stats[(int64_t)p.hq * p.rows_total + si] = end.l;
         } else {
           ws.ml[(int64_t)pc.slot * kUnitRows + row_in_unit] = make_float2(m, l);
         }

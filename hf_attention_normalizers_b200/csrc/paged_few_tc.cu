@@ -15,7 +15,10 @@
 //
 // The reference m of a row follows the maximum lazily and only when a score
 // passes it by 2^8, which one vote of the four warps finds; a decoded row
-// seldom takes that path.  The CTAs walk equal stretches of all key tiles of
+// seldom takes that path.  It starts at the implicit zero logit in bfloat16,
+// whose exponents reach as far as float32's.  In float16, where P below 2^-14
+// loses bits and vanishes below 2^-25, it starts 2^8 under the maximum of the
+// piece's first tile, which may lie far below zero, and follows past 2^15.  The CTAs walk equal stretches of all key tiles of
 // the batch (paged_walk.cuh).
 //
 // Measured: 8 sequences of 32k keys, one token each, 8 KV heads of 128: 1.07 GB
@@ -39,7 +42,12 @@ namespace {
 using namespace tc;
 
 constexpr int kFewThreads = 192;
-constexpr float kRescale = 8.f;
+
+// A row's reference moves when a score passes it by kRescale octaves.  float16:
+// P stays below 2^15, and a new reference lies kHeadroom16 octaves below the
+// maximum (paged_walk.cuh).
+template <bool BF16>
+constexpr float kRescale = BF16 ? 8.f : 15.f;
 
 constexpr int kSumStride = 132;  // floats; rows of 128 start in different banks
 
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
         for (int e = 0; e < NC; ++e) {
           x[e] = e >= lo && e < rows ? __uint_as_float(sx[e]) * zs : kNegInf;
-          high |= x[e] > m[e] + kRescale;
+          high |= x[e] > m[e] + kRescale<BF16>;
         }
         if (scores != nullptr && key < u.g.k_len) {
           const int keep = score_floats(c);
@@ -266,13 +274,13 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           for (int e = 0; e < NC; e += 4)
             if (e < keep) dst[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         }
-        if (named_bar_or(1, 128, high)) {
-          // some row passed its reference: the tile's row maxima over the four warps
+        if (named_bar_or(1, 128, high || (!BF16 && t == 0))) {
+          // some row passed its reference (or has none yet): the tile's row maxima over the four warps
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
-            // only maxima above m + 2^3 > 0 matter, and positive floats compare as integers
-            const int w = __reduce_max_sync(0xffffffffu, __float_as_int(fmaxf(x[e], 0.f)));
-            if (lane == 0) red[warp * NC + e] = __int_as_float(w);
+            // bfloat16: only maxima above m + 2^3 > 0 matter, and positive floats compare as integers
+            const int w = __reduce_max_sync(0xffffffffu, BF16 ? __float_as_int(fmaxf(x[e], 0.f)) : ordered_int(x[e]));
+            if (lane == 0) red[warp * NC + e] = __int_as_float(BF16 ? w : ordered_int(__int_as_float(w)));
           }
           named_bar_sync(1, 128);
           float alpha[NC];
@@ -280,9 +288,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           for (int e = 0; e < NC; ++e) {
             const float top = fmaxf(fmaxf(red[e], red[NC + e]), fmaxf(red[2 * NC + e], red[3 * NC + e]));
             alpha[e] = 1.f;
-            if (top > m[e] + kRescale) {
-              alpha[e] = exp2f(m[e] - top);
-              m[e] = top;
+            if (top > m[e] + kRescale<BF16> || (!BF16 && t == 0)) {
+              const float ref = BF16 ? top : reference16(top);
+              alpha[e] = exp2f(m[e] - ref);
+              m[e] = ref;
               l[e] *= alpha[e];
             }
           }
@@ -356,14 +365,14 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
       for (int e = 0; e < NC; ++e) {
         if (e < rows) {
-          float sum = red[e];
+          const float sum = red[e];
           if (pc.whole) {
-            sum += exp2f(-m[e]);  // the implicit zero logit
+            const RowEnd end = end_of_row<BF16>(m[e], sum);
             if (r < HD)
-              static_cast<T*>(p.o)[tok * p.o_st + (int64_t)h * p.o_sh + r] = from_f32<T>(__uint_as_float(o[e]) * (1.f / sum));
+              static_cast<T*>(p.o)[tok * p.o_st + (int64_t)h * p.o_sh + r] = from_f32<T>(__uint_as_float(o[e]) * end.inv);
             if (r == 0) {
-              p.stats[(int64_t)h * p.rows_total + tok] = m[e];
-              p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = sum;
+              p.stats[(int64_t)h * p.rows_total + tok] = end.m;
+              p.stats[(int64_t)(p.hq + h) * p.rows_total + tok] = end.l;
             }
           } else {
             const int64_t at = (int64_t)pc.slot * ws.rows + e;

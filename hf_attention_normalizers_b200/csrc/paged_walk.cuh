@@ -142,6 +142,40 @@ class Walk {
   int per_, at_, end_, u0_, group_;
 };
 
+// The softmax1 kernels exponentiate a row against a reference m that follows its
+// maximum lazily, and round P to the inputs' type.  In float16 the reference is
+// kept kHeadroom16 octaves below the maximum that set it: P of that key is 2^8,
+// and P down to 2^-22 of it is a normal number.  Rows that attend to almost
+// nothing (all scores far below the implicit zero logit) so have references
+// below zero.  kLowestRef keeps 2^-m finite: such a row's output is zero in
+// float16 as well.  top: the maximum, -inf when there is none (m: 0).
+constexpr float kHeadroom16 = 8.f, kLowestRef = -100.f;
+__device__ __forceinline__ float reference16(float top) {
+  return top > kNegInf ? fmaxf(top - kHeadroom16, kLowestRef) : 0.f;
+}
+
+// Integers in the order of the floats; its own inverse on the bits.
+__device__ __forceinline__ int ordered_int(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+
+// Statistics (reference max(m, 0), denominator with the implicit zero logit) of
+// a row with reference m and sum l, and the factor of its unscaled output.
+struct RowEnd {
+  float m, l, inv;
+};
+template <bool BF16>
+__device__ __forceinline__ RowEnd end_of_row(float m, float l) {
+  if (BF16) {  // (m >= 0)
+    l += exp2f(-m);
+    return RowEnd{m, l, 1.f / l};
+  }
+  const float top = fmaxf(m, 0.f), scale = exp2f(m - top);
+  l = l * scale + exp2f(-top);
+  return RowEnd{top, l, scale / l};
+}
+
 // Joins the pieces of split units: one block per (token, KV head) and its G rows.
 // Tokens that no sequence owns get theirs here.
 template <int HD, typename T>

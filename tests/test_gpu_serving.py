@@ -356,6 +356,39 @@ def test_rows_of_no_sequence_are_zero(new, lens, kw, norm):
     assert serving.device_status() == 0
 
 
+def _low_scores(b, profile):
+    """Scores of the given profile (natural units, along the keys) for every row, values that do not cancel."""
+    b.query.zero_()
+    b.query[..., 0] = 4.0
+    for r in b.rows:
+        b.key_cache[r] = torch.randn(b.key_cache[r].shape, generator=torch.Generator().manual_seed(7)).to(b.dtype)
+        b.key_cache[r, :, 0] = (profile(len(r)) / (4.0 * b.dim ** -0.5)).to(b.dtype)[:, None]
+        b.value_cache[r] = b.value_cache[r].abs()
+    b.d_query, b.d_key, b.d_value = b.query.cuda(), b.key_cache.cuda(), b.value_cache.cuda()
+
+
+LOW_SCORES = {
+    "even": lambda n: torch.full((n,), -17.0),
+    "range": lambda n: -18.0 + 6.0 * torch.rand(n, generator=torch.Generator().manual_seed(8)),
+    "lower": lambda n: torch.full((n,), -22.0),
+    "lowest": lambda n: torch.full((n,), -90.0),
+    "rising": lambda n: torch.linspace(-24.0, 9.0, n),
+    "falling": lambda n: torch.linspace(9.0, -24.0, n),
+    "one high key": lambda n: torch.where(torch.arange(n) == n - 70, -3.0, -17.0),
+}
+
+
+@pytest.mark.parametrize("profile", LOW_SCORES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [[1, 3], [70, 2]])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rows_that_attend_to_almost_nothing(dtype, new, dim, profile):
+    """softmax1 with every score far below its implicit zero logit: the small outputs keep their precision."""
+    b = Batch(new, [6000, 900], seed=56, hkv=1, dim=dim, dtype=dtype, stale=0.0)
+    _low_scores(b, LOW_SCORES[profile])
+    _chunk_case(b, "softmax1")
+
+
 # ---------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------
