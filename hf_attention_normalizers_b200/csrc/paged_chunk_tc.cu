@@ -56,6 +56,10 @@ constexpr int kChunkThreads = 352;
 constexpr int kMaxRing = 8;
 template <bool BF16>
 constexpr float kHighSum = BF16 ? 4096.f : 32768.f;  // (also keeps P below float16's 65504)
+// Factor of s - tau: float16 takes the sparse normalizers' P (at most 1) times
+// 2^14, since supports of tens of thousands of keys lie among its subnormals.
+template <bool BF16, int NORM>
+constexpr float kLift = BF16 ? 1.f : (NORM == HFAN_SPARSEMAX ? 0x1p14f : 0x1p7f);
 constexpr int kUnitRows = 2 * kTileRows;
 constexpr int kHalfKeys = kTileKeys / 2;
 
@@ -391,7 +395,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (!ok) break;
             l += sum;
           } else {
-            const uint64_t zs2 = f2_pack(zs, zs), nt2 = f2_pack(-m, -m);
+            const float zl = zs * kLift<BF16, NORM>, tl = m * kLift<BF16, NORM>;
+            const uint64_t zs2 = f2_pack(zl, zl), nt2 = f2_pack(-tl, -tl);
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               const uint64_t y = ffma2(f2_pack(s[e], s[e + 1]), zs2, nt2);
@@ -416,7 +421,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       tc_fence_after();
       const int row_in_unit = q * kTileRows + r;
       const RowEnd end = end_of_row<BF16>(m, l);
-      const float inv = NORM == HFAN_SOFTMAX1 ? end.inv : 1.f;  // (of whole pieces)
+      // (pieces of the sparse normalizers are whole)
+      const float inv = NORM == HFAN_SOFTMAX1 ? (pc.whole ? end.inv : 1.f) : (BF16 ? 1.f : 0x1p-14f);
       T* dst = static_cast<T*>(p.o) + (int64_t)(u.g.q_start + i) * p.o_st + (int64_t)h * p.o_sh;
       float* part = ws.o + ((int64_t)pc.slot * kUnitRows + row_in_unit) * HD;
 #pragma unroll 1

@@ -389,6 +389,16 @@ def test_rows_that_attend_to_almost_nothing(dtype, new, dim, profile):
     _chunk_case(b, "softmax1")
 
 
+@pytest.mark.parametrize("norm", ["sparsemax", "entmax15"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_supports_of_very_many_keys(norm, dtype):
+    """Even rows over a long context: every probability lies among float16's subnormal numbers."""
+    b = Batch([1], [83677], seed=62, group=1, hkv=1, dim=64, page=64, dtype=dtype, stale=0.0)
+    b.value_cache = b.value_cache.abs()
+    b.d_value = b.value_cache.cuda()
+    _chunk_case(b, norm, scale=1e-12)
+
+
 # ---------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------
