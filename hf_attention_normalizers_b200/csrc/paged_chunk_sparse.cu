@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t p2 = f2_pack(pr, pr);
             uint4 x[V];
 #pragma unroll
-            for (int y = 0; y < V; ++y) x[y] = __ldg(v + y);
+            for (int y = 0; y < V; ++y) x[y] = v[y];  // (coherent: an append or eviction may end during this launch)
 #pragma unroll
             for (int y = 0; y < V; ++y) {
               acc[4 * y + 0] = ffma2(p2, unpack2<BF16>(x[y].x), acc[4 * y + 0]);

@@ -577,6 +577,33 @@ def test_offsets_past_32_bits():
     assert serving.device_status() == 0
 
 
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 1, 90]])
+def test_pages_rewritten_back_to_back(norm, new):
+    """Each call reads what the one before it wrote into the same pages, launched while that one still runs."""
+    rows = torch.randn(12, sum(new), 2, 2, 128, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+
+    def run(pause):
+        b = Batch(new, [300, 700, 260], seed=63, gain=2.0)
+        outs = []
+        for x in rows:
+            serving.paged_append(x[:, 0], x[:, 1], b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page,
+                                 key_weights=b.d_weights)
+            pause()
+            outs.append(b.chunk(norm, key_weights=b.d_weights))
+            pause()
+        for budget in range(240, 100, -20):
+            b.d_seq, _ = serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, budget, recent=95)
+            pause()
+            outs.append(b.chunk(norm, key_weights=b.d_weights))
+            pause()
+        return outs + [b.d_weights]
+
+    for got, want in zip(run(lambda: None), run(torch.cuda.synchronize)):
+        assert torch.equal(got, want)
+    assert serving.device_status() == 0
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
