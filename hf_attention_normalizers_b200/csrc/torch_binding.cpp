@@ -119,6 +119,15 @@ struct Weights {
   }
 };
 
+// A tensor that the kernels wrote in place: autograd finds out by its version
+// when it had saved it.  (Inference tensors have none.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject* weights) {
+  if (weights != Py_None) written(tensor(weights));
+}
+
 // (key, value, key_cache, value_cache, block_table, cu_seqlens, lengths, page_size, max_q, key_weights)
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 10, [&]() -> PyObject* {
@@ -147,6 +156,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(fn_append(&d, view(key), view(value), view(kc), view(vc), w.data, w.ld,
                     c10::cuda::getCurrentCUDAStream(key.device().index()).stream()),
           "hfan_paged_append");
+    written(kc);
+    written(vc);
+    written(a[9]);
     Py_RETURN_NONE;
   });
 }
@@ -189,6 +201,7 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    bytes > 0 ? ws.data_ptr() : nullptr, bytes > 0 ? bytes : 0,
                    c10::cuda::getCurrentCUDAStream(q.device().index()).stream()),
           "hfan_paged_chunk_fwd");
+    written(a[12]);
     return Py_BuildValue("NN", THPVariable_Wrap(o), THPVariable_Wrap(stats));
   });
 }
@@ -220,6 +233,9 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(fn_evict(&d, view(kc), view(vc), w.data, w.ld, budget, int32(a[8]), kept.data_ptr<int32_t>(),
                    cut.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(kc.device().index()).stream()),
           "hfan_paged_evict");
+    written(kc);
+    written(vc);
+    written(a[2]);
     return Py_BuildValue("NN", THPVariable_Wrap(cut), THPVariable_Wrap(kept));
   });
 }

@@ -616,6 +616,44 @@ def test_gradients_are_refused():
         assert torch.isfinite(b.chunk("softmax1")).all()
 
 
+@pytest.mark.parametrize("norm", NORMS)
+def test_written_tensors_raise_their_versions(norm):
+    """Autograd has to notice that a cache it saved was written."""
+    b = Batch([3, 1], [60, 40], seed=58)
+    new = torch.randn(4, b.hkv, b.dim, device="cuda").to(b.dtype)
+
+    def versions():
+        return [t._version for t in (b.d_key, b.d_value, b.d_weights)]
+
+    was = versions()
+    serving.paged_append(new, new, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page, key_weights=b.d_weights)
+    now = versions()
+    assert all(a > w for a, w in zip(now, was))
+    b.chunk(norm, key_weights=b.d_weights)
+    assert versions()[:2] == now[:2] and versions()[2] > now[2]
+    was = versions()
+    serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, 20)
+    assert all(a > w for a, w in zip(versions(), was))
+
+    factor = torch.ones((), device="cuda", dtype=b.dtype, requires_grad=True)
+    y = b.d_key * factor  # saves the cache
+    with torch.no_grad():
+        serving.paged_append(new, new, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_inference_mode():
+    """Tensors without a version counter."""
+    with torch.inference_mode():
+        b = Batch([3, 1], [60, 40], seed=59)
+        new = torch.randn(4, b.hkv, b.dim, device="cuda").to(b.dtype)
+        serving.paged_append(new, new, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page, key_weights=b.d_weights)
+        b.key_cache, b.value_cache, b.weights = b.d_key.cpu(), b.d_value.cpu(), b.d_weights.cpu()
+        _chunk_case(b, "softmax1")
+        serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, 20)
+
+
 def test_tensors_elsewhere_are_refused():
     b = Batch([2], [20], seed=41)
     with pytest.raises(ValueError, match="requires CUDA"):
