@@ -485,9 +485,10 @@ torch.library.register_autograd("hfan::paged_fwd", _paged_backward, setup_contex
 #
 # The plain functions launch the kernels (through csrc/torch_binding.cpp: a
 # decode step makes these calls in every layer, and ctypes would cost more than
-# the kernels); the custom ops of the same name wrap them for traced graphs.
-# The op dispatch costs as much host time as the whole launch, so eager callers
-# (serving.py) use the functions.
+# the kernels); the custom ops of the same name wrap them for whoever watches or
+# replaces calls (traced graphs, dispatch modes, fake tensors, the profiler).
+# The op dispatch costs as much host time as the whole launch, so other eager
+# calls (serving.py) use the functions.
 # ---------------------------------------------------------------------------
 def launch_paged_append(key: Tensor, value: Tensor, key_cache: Tensor, value_cache: Tensor, block_table: Tensor,
                         cu_seqlens: Tensor, seq_lens: Tensor, page_size: int, max_q: int,

@@ -86,13 +86,23 @@ def _check_rows(rows, key_cache, cu_seqlens, block_table, name) -> None:
         raise ValueError("New tokens and cache head dimensions must match.")
 
 
-def _check_placement(*tensors) -> None:
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _check_placement(*tensors) -> bool:
+    """Returns whether somebody listens for the call: it is then dispatched as a custom op, else launched directly
+    (the dispatch costs as much host time as the launch)."""
     where = tensors[0].get_device()
+    observed = (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+                or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._autograd._profiler_enabled())
     for t in tensors:
-        if t is not None and t.get_device() != where:
-            raise ValueError("All tensors must be on one device.")
+        if t is not None:
+            if t.get_device() != where:
+                raise ValueError("All tensors must be on one device.")
+            observed = observed or type(t) not in _PLAIN
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError("Paged serving is inference only: call it under torch.no_grad() or detach its inputs.")
+    return observed
 
 
 def _bound(given: Optional[int], most: int, name: str) -> int:
@@ -119,8 +129,8 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     if key.shape[1] != key_cache.shape[1]:
         raise ValueError("New keys and cache must have the same KV heads.")
     _check_rows(key, key_cache, cu_seqlens, block_table, "cu_seqlens")
-    _check_placement(key_cache, value_cache, key, value, block_table, cu_seqlens, sequence_lengths, key_weights)
-    call = ops.paged_append if torch.compiler.is_compiling() else ops.launch_paged_append
+    observed = _check_placement(key_cache, value_cache, key, value, block_table, cu_seqlens, sequence_lengths, key_weights)
+    call = ops.paged_append if observed else ops.launch_paged_append
     call(key, value, key_cache, value_cache, block_table, cu_seqlens, sequence_lengths, int(block_size), key.shape[0],
          key_weights)
 
@@ -147,14 +157,14 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     if query.shape[1] % key_cache.shape[1] != 0:
         raise ValueError("query heads must be divisible by KV heads.")
     _check_rows(query, key_cache, cu_seqlens_q, block_table, "cu_seqlens_q")
-    _check_placement(key_cache, value_cache, query, block_table, cu_seqlens_q, sequence_lengths, key_weights)
+    observed = _check_placement(key_cache, value_cache, query, block_table, cu_seqlens_q, sequence_lengths, key_weights)
     norm = N.NORMALIZER_IDS.get(normalizer) if isinstance(normalizer, str) else None
     if norm is None:
         norm = N.NORMALIZER_IDS[_normalizer_name(normalizer)]
     max_q = _bound(max_seqlen_q, query.shape[0], "max_seqlen_q")
     max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
     actual_scale = query.shape[-1] ** -0.5 if scale is None else float(scale)
-    call = ops.paged_chunk_fwd if torch.compiler.is_compiling() else ops.launch_paged_chunk_fwd
+    call = ops.paged_chunk_fwd if observed else ops.launch_paged_chunk_fwd
     return call(query, key_cache, value_cache, block_table, cu_seqlens_q, sequence_lengths, int(block_size), max_q, max_k,
                 norm, actual_scale, bool(is_causal), key_weights)[0]
 
@@ -180,9 +190,9 @@ def paged_evict(key_cache: torch.Tensor, value_cache: torch.Tensor, key_weights:
         raise ValueError("budget must be positive.")
     if recent < 0:
         raise ValueError("recent must not be negative.")
-    _check_placement(key_cache, value_cache, block_table, sequence_lengths, key_weights)
+    observed = _check_placement(key_cache, value_cache, block_table, sequence_lengths, key_weights)
     max_k = _bound(max_seqlen_k, block_table.shape[1] * block_size, "max_seqlen_k")
-    call = ops.paged_evict if torch.compiler.is_compiling() else ops.launch_paged_evict
+    call = ops.paged_evict if observed else ops.launch_paged_evict
     return call(key_cache, value_cache, key_weights, block_table, sequence_lengths, int(block_size), max_k, int(budget),
                 int(recent))
 

@@ -654,6 +654,33 @@ def test_inference_mode():
         serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, 20)
 
 
+def test_dispatch_modes_and_the_profiler_see_the_calls():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    b = Batch([3, 1], [60, 40], seed=60)
+    new = torch.randn(4, b.hkv, b.dim, device="cuda").to(b.dtype)
+
+    def step():
+        serving.paged_append(new, new, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page, key_weights=b.d_weights)
+        b.chunk("softmax1", key_weights=b.d_weights)
+        serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq, b.page, 20)
+
+    names = ["hfan::paged_append", "hfan::paged_chunk_fwd", "hfan::paged_evict"]
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    with Log():
+        step()
+    assert [n for n in seen if n.startswith("hfan::")] == names
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        step()
+    assert set(names) <= {e.name for e in prof.events()}
+
+
 def test_tensors_elsewhere_are_refused():
     b = Batch([2], [20], seed=41)
     with pytest.raises(ValueError, match="requires CUDA"):

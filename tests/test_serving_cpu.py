@@ -77,3 +77,21 @@ def test_evict_requests_are_refused_on_the_host(budget, recent, ld, msg):
     lib, t, one = N.lib(), N.HfanTensor(None, 0, 0, 0), ctypes.c_void_p(1)
     assert lib.hfan_paged_evict(ctypes.byref(_desc(cu_seqlens_q=None)), t, t, one, ld, budget, recent, one, one, None) == 1
     assert msg in lib.hfan_last_error().decode()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_fake_tensors(grad):
+    """Outside torch.compile: shapes come from the custom ops, nothing is launched."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(), torch.set_grad_enabled(grad):
+        def make(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        kc, vc, w, table = make(64, 2, 64), make(64, 2, 64), make(2, 64, dtype=torch.float32), make(2, 2, dtype=torch.int32)
+        cu, lens = make(3, dtype=torch.int32), make(2, dtype=torch.int32)
+        assert serving.paged_append(make(3, 2, 64), make(3, 2, 64), kc, vc, table, cu, lens, 16, key_weights=w) is None
+        out = serving.paged_chunk_attention(make(3, 4, 64), kc, vc, table, cu, lens, 16, key_weights=w)
+        assert out.shape == (3, 4, 64) and out.dtype is torch.bfloat16 and out.device.type == "cuda"
+        lens, kept = serving.paged_evict(kc, vc, w, table, lens, 16, 10)
+        assert lens.shape == (2,) and kept.shape == (2, 2, 10) and kept.dtype is torch.int32
