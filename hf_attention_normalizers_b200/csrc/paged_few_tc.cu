@@ -77,8 +77,13 @@ static_assert(FewLayout<128, 16>::TOTAL <= 232448 && FewLayout<128, 32>::TOTAL <
                   FewLayout<64, 16>::TOTAL <= 232448 && FewLayout<64, 32>::TOTAL <= 232448,
               "more shared memory than a block can have");
 
-// Scores kept of a key: its packed rows, rounded up to whole vectors.
-__host__ __device__ __forceinline__ int score_floats(const ChunkPlan& c) { return (c.tpb * c.group + 3) & ~3; }
+// Kept scores: [KV head][key][score_floats(rows of the group)] for every group of
+// tokens, rows rounded up to whole vectors.  A token has room for the rounded
+// rows of its own, which suffices for groups of any size.
+__host__ __device__ __forceinline__ int score_floats(int rows) { return (rows + 3) & ~3; }
+__device__ __forceinline__ int64_t score_index(const AttnParams& p, const ChunkPlan& c, int64_t tok, int kvh, int key, int rows) {
+  return tok * p.hkv * p.len_k * score_floats(c.group) + ((int64_t)kvh * p.len_k + key) * score_floats(rows);
+}
 
 __device__ __forceinline__ void fail(const AttnParams& p, FewBars* s) {
   s->abort = 1;
@@ -242,6 +247,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       const Unit& u = walk.u;
       const Piece& pc = walk.piece;
       const int rows = u.ntok * c.group;
+      const int keep = score_floats(rows);
+      float* kept = scores + score_index(p, c, u.g.q_start + u.tok0, u.kvh, 0, rows);
       float m[NC], l[NC];
 #pragma unroll
       for (int x = 0; x < NC; ++x) m[x] = l[x] = 0.f;
@@ -267,9 +274,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           high |= x[e] > m[e] + kRescale<BF16>;
         }
         if (scores != nullptr && key < u.g.k_len) {
-          const int keep = score_floats(c);
-          float4* dst = reinterpret_cast<float4*>(
-              scores + (((int64_t)(u.g.q_start + u.tok0) * p.hkv + u.kvh) * p.len_k + key) * keep);
+          float4* dst = reinterpret_cast<float4*>(kept + (int64_t)key * keep);
 #pragma unroll
           for (int e = 0; e < NC; e += 4)
             if (e < keep) dst[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
@@ -426,8 +431,7 @@ __global__ void __launch_bounds__(256) few_weights_kernel(const AttnParams p, co
     __syncthreads();
     // keys that no row of the group sees have no tile, hence no scores
     if (key >= g.k_len || (p.causal && key > g.shift + tok0 + rows / c.group - 1)) continue;
-    const float4* s = reinterpret_cast<const float4*>(
-        scores + (((int64_t)(g.q_start + tok0) * p.hkv + kvh) * p.len_k + key) * score_floats(c));
+    const float4* s = reinterpret_cast<const float4*>(scores + score_index(p, c, g.q_start + tok0, kvh, key, rows));
 #pragma unroll
     for (int e = 0; e < NC; e += 4) {
       if (e >= rows) break;
@@ -477,7 +481,7 @@ int few_columns(const AttnParams& p) {
 constexpr int64_t kFewScoreBytes = 1ll << 30;  // scores kept at most; beyond, the weights read K again
 
 static int64_t score_bytes(const AttnParams& p, const ChunkPlan& c) {
-  return (int64_t)p.rows_total * p.hkv * p.len_k * score_floats(c) * 4;
+  return (int64_t)p.rows_total * p.hkv * p.len_k * score_floats(c.group) * 4;
 }
 
 bool chunk_few_applies(const AttnParams& p, const ChunkPlan& c, bool weights) {

@@ -79,6 +79,14 @@ def test_evict_requests_are_refused_on_the_host(budget, recent, ld, msg):
     assert msg in lib.hfan_last_error().decode()
 
 
+def test_workspace_holds_each_score_once():
+    """Kept scores of 8-token chunks: four bytes a (row, key)."""
+    lib = N.lib()
+    d = _desc(batch=8, heads_q=8, heads_kv=2, total_q=64, max_len_q=8, max_blocks=512, max_len_k=8192)
+    size = [lib.hfan_paged_chunk_workspace_bytes(ctypes.byref(d), w) for w in (0, 1)]
+    assert 0 < size[0] and size[1] - size[0] == 64 * 8 * 8192 * 4
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_fake_tensors(grad):
     """Outside torch.compile: shapes come from the custom ops, nothing is launched."""
