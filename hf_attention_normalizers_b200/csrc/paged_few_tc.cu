@@ -15,11 +15,11 @@
 //
 // The reference m of a row follows the maximum lazily and only when a score
 // passes it by 2^8, which one vote of the four warps finds; a decoded row
-// seldom takes that path.  It starts at the implicit zero logit in bfloat16,
-// whose exponents reach as far as float32's.  In float16, where P below 2^-14
-// loses bits and vanishes below 2^-25, it starts 2^8 under the maximum of the
-// piece's first tile, which may lie far below zero, and follows past 2^15.  The CTAs walk equal stretches of all key tiles of
-// the batch (paged_walk.cuh).
+// seldom takes that path. It starts at the implicit zero logit in bfloat16,
+// whose exponents reach as far as float32's. In float16, where P below 2^-14
+// loses bits and vanishes below 2^-25, a row whose first tile stays below that
+// logit starts 2^8 under its maximum there, and all follow past 2^15. The CTAs
+// walk equal stretches of all key tiles of the batch (paged_walk.cuh).
 //
 // Measured: 8 sequences of 32k keys, one token each, 8 KV heads of 128: 1.07 GB
 // in 178 us, 6.0 TB/s of DRAM reads (0.92 of a copy); 4 sequences of up to 2k
@@ -279,8 +279,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           for (int e = 0; e < NC; e += 4)
             if (e < keep) dst[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         }
-        if (named_bar_or(1, 128, high || (!BF16 && t == 0))) {
-          // some row passed its reference (or has none yet): the tile's row maxima over the four warps
+        if (!BF16 && t == 0) {
+          // rows that the warp's keys leave below the implicit zero logit
+          uint32_t seen = 0u, above = 0u;
+#pragma unroll
+          for (int e = 0; e < NC; ++e) {
+            seen |= x[e] > kNegInf ? 1u << e : 0u;
+            above |= x[e] >= 0.f ? 1u << e : 0u;
+          }
+          high |= (__reduce_or_sync(0xffffffffu, seen) & ~__reduce_or_sync(0xffffffffu, above)) != 0u;
+        }
+        if (named_bar_or(1, 128, high)) {
+          // some row passed its reference (float16: or may start far below it): the tile's row maxima over the four warps
 #pragma unroll
           for (int e = 0; e < NC; ++e) {
             // bfloat16: only maxima above m + 2^3 > 0 matter, and positive floats compare as integers
