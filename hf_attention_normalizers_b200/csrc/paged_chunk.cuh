@@ -24,11 +24,14 @@ struct ChunkPlan {
   int pairs;     // upper bound of the tile pairs of all sequences
 };
 
-// Tokens of sequence b and the first of them, clamped as geometry() does.
+// Tokens of sequence b and the first of them, clamped and recorded as geometry()
+// does (which nobody calls for a sequence that decreasing offsets leave empty).
 __device__ __forceinline__ int chunk_tokens(const AttnParams& p, int b, int* start) {
-  const int s = min(max(p.cu_q[b], 0), p.rows_total);
+  const int s0 = p.cu_q[b], e0 = p.cu_q[b + 1];
+  const int s = min(max(s0, 0), p.rows_total), e = min(max(e0, s), p.rows_total);
+  if ((s != s0 || e != e0) && p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevBadLength);
   *start = s;
-  return min(max(p.cu_q[b + 1], s), p.rows_total) - s;
+  return e - s;
 }
 
 // The x-th group of `per` tokens over all sequences (the last of a sequence

@@ -553,6 +553,21 @@ def test_bad_offsets_stay_inside_the_packed_rows(norm, new):
     assert serving.device_status() == 0
 
 
+@pytest.mark.parametrize("norm", NORMS)
+@pytest.mark.parametrize("kw", [dict(), dict(dtype=torch.float32)])
+@pytest.mark.parametrize("new", [[1, 2], [60, 70], [3] + [0] * 40 + [1]])
+def test_decreasing_offsets_are_recorded(new, kw, norm):
+    """A sequence whose offsets decrease has no tokens, rows before both are served, and the status tells."""
+    b = Batch(new, [200] * len(new), seed=64, **kw)
+    want, tol, _, _ = b.expected(norm)
+    serving.device_status()
+    for end in (new[0] - 1, -5):
+        b.d_cu[-1] = end
+        out = b.chunk(norm)
+        assert serving.device_status() == 3
+        _check(out[:new[0] - 1], want[:new[0] - 1], tol[:new[0] - 1], norm) if end >= 0 and new[0] > 1 else None
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^32 bytes and 2^31 elements, its pages in use at the far end: the same bits as in a small one."""
     small = Batch([70, 1, 3], [400, 600, 131], seed=50, hkv=8, group=2, interleave=True, stale=0.0)
