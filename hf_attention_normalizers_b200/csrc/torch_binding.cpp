@@ -52,8 +52,11 @@ int32_t size32(int64_t v) {
   return (int32_t)v;
 }
 
+// 64-bit integers saturate: cut to 32 bits, a wild length or page id could pass
+// for a valid one, which the kernels then would not record.
 at::Tensor ints(const at::Tensor& t) {
-  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+  if (t.scalar_type() == at::kInt) return t.contiguous();
+  return t.clamp(at::Scalar(INT32_MIN), at::Scalar(INT32_MAX)).to(at::kInt).contiguous();
 }
 at::Tensor rows(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 hfan_tensor view(const at::Tensor& t) { return hfan_tensor{t.data_ptr(), 0, t.stride(1), t.stride(0)}; }

@@ -631,6 +631,29 @@ def test_gradients_are_refused():
         assert torch.isfinite(b.chunk("softmax1")).all()
 
 
+def test_64_bit_integers_past_32_bits_are_recorded():
+    """Lengths, offsets and page ids that a cut to 32 bits would turn into valid ones."""
+    b = Batch([3, 1], [60, 40], seed=61)
+    out = b.chunk("softmax1")
+    b.d_table, b.d_cu, b.d_seq = b.d_table.long(), b.d_cu.long(), b.d_seq.long()
+    assert torch.equal(b.chunk("softmax1"), out) and serving.device_status() == 0
+    for field, at, status in (("d_table", (0, 0), 1), ("d_seq", 0, 3), ("d_cu", 2, 3)):
+        t = getattr(b, field)
+        for by in (2 ** 32, -2 ** 32):
+            t[at] += by
+            b.chunk("softmax1")
+            assert serving.device_status() == status, field
+            t[at] -= by
+    new = torch.randn(4, b.hkv, b.dim, device="cuda").to(b.dtype)
+    key = b.d_key.clone()
+    b.d_table[:, :2] += 2 ** 32
+    serving.paged_append(new, new, b.d_key, b.d_value, b.d_table, b.d_cu, b.d_seq, b.page)
+    assert torch.equal(b.d_key.nan_to_num(), key.nan_to_num()) and serving.device_status() == 1
+    b.d_table[:, :2] -= 2 ** 32
+    lens, _ = serving.paged_evict(b.d_key, b.d_value, b.d_weights, b.d_table, b.d_seq + 2 ** 32, b.page, 50)
+    assert lens.tolist() == [50, 50] and serving.device_status() == 3
+
+
 @pytest.mark.parametrize("norm", NORMS)
 def test_written_tensors_raise_their_versions(norm):
     """Autograd has to notice that a cache it saved was written."""
