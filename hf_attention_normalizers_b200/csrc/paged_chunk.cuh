@@ -24,14 +24,22 @@ struct ChunkPlan {
   int pairs;     // upper bound of the tile pairs of all sequences
 };
 
-// Tokens of sequence b and the first of them, clamped and recorded as geometry()
-// does (which nobody calls for a sequence that decreasing offsets leave empty).
+// Tokens of sequence b and the first of them, clamped as geometry() does.
 __device__ __forceinline__ int chunk_tokens(const AttnParams& p, int b, int* start) {
-  const int s0 = p.cu_q[b], e0 = p.cu_q[b + 1];
-  const int s = min(max(s0, 0), p.rows_total), e = min(max(e0, s), p.rows_total);
-  if ((s != s0 || e != e0) && p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevBadLength);
+  const int s = min(max(p.cu_q[b], 0), p.rows_total);
   *start = s;
-  return e - s;
+  return min(max(p.cu_q[b + 1], s), p.rows_total) - s;
+}
+
+// Records offsets that chunk_tokens clamped, as geometry() does (which nobody
+// calls for a sequence that they leave empty).  For threads with nothing else to
+// do: in the searches of all warps the test cost a small decode 0.5 us.
+__device__ __forceinline__ void record_bad_offsets(const AttnParams& p, int thread, int threads) {
+  for (int b = thread; b < p.batch; b += threads) {
+    int s;
+    const int n = chunk_tokens(p, b, &s);
+    if ((s != p.cu_q[b] || s + n != p.cu_q[b + 1]) && p.dev_status) atomicCAS(p.dev_status, kDevOk, kDevBadLength);
+  }
 }
 
 // The x-th group of `per` tokens over all sequences (the last of a sequence

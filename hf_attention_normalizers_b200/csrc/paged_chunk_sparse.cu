@@ -153,12 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const UnownedRows rest(p);
   for (int x = blockIdx.x; x < rest.count; x += gridDim.x)
     store_empty_rows<T, uint4>(p, rest.at(x), blockIdx.y * c.group, c.group);
-  // (a unit's search ends at its sequence: one CTA looks at all offsets)
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int x = threadIdx.x; x < p.batch; x += kThreads) {
-      int start;
-      chunk_tokens(p, x, &start);
-    }
+  if (warp == 11 && blockIdx.x == 0 && blockIdx.y == 0) record_bad_offsets(p, lane, 32);
   int b, pair;
   const int unit = blockIdx.x / ranks;
   if (!find_group(p, 2 * c.tpb, unit, &b, &pair)) return;  // the whole cluster alike

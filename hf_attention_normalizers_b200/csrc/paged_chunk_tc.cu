@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else {
     // ------------------------------------------------------------ row warps
     const int q = warp >> 2, r = threadIdx.x & 127;
+    if (NORM == HFAN_SOFTMAX1 && blockIdx.x == gridDim.x - 1) record_bad_offsets(p, threadIdx.x, 256);
     const int rt = r / c.group, rg = r - rt * c.group;  // token of the tile, head of the group
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lane_addr + q * 128, o_col = tmem + lane_addr + 256 + q * 128;

@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   } else {
     // ------------------------------------------------------------ softmax
     const int r = threadIdx.x;  // key of the tile; head dim of O^T
+    if (blockIdx.x == gridDim.x - 1) record_bad_offsets(p, r, 128);
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     const float zs = p.scale * kLog2e;
     float* red = reinterpret_cast<float*>(smem + L::RED);
