@@ -28,6 +28,10 @@
 // float16 it starts 2^8 below the maximum of the piece's first half and moves
 // past a sum of 2^15, see reference16 (paged_walk.cuh).
 //
+// P is rounded to the inputs' type, at most half a unit of each p beside the
+// rounding of the result: a second 16-bit part for the rest would repeat the
+// P V products, half of the tensor pipe's work here.
+//
 // Measured: 1024 tokens on 32k keys (32 / 8 heads of 128), 0.55 TFLOP: 0.52 ms
 // from a cool start, 0.64 ms in a row, where the 1000 W limit holds the clock at
 // 1.6 GHz; tensor pipe busy 49% of the cycles.  Passing tiles through without

@@ -21,6 +21,13 @@
 // logit starts 2^8 under its maximum there, and all follow past 2^15. The CTAs
 // walk equal stretches of all key tiles of the batch (paged_walk.cuh).
 //
+// P enters P V as two 16-bit parts, P rounded and what the rounding left, so
+// that only the result is rounded (one part: output errors 1.5 times those of
+// a float32 computation that rounds its result).  The tensor pipe has room: 8
+// sequences of 32k keys take 191.0 us with two parts and 190.3 with one, 16
+// chunks of 8 tokens on 8k keys 123.2 and 121.0 (medians of graph launches, L2
+// flushed).
+//
 // Measured: 8 sequences of 32k keys, one token each, 8 KV heads of 128: 1.07 GB
 // in 178 us, 6.0 TB/s of DRAM reads (0.92 of a copy); 4 sequences of up to 2k
 // keys: 12 us, of which setting up (barriers, TMEM, the walk) takes 2 and the
@@ -53,13 +60,13 @@ constexpr int kSumStride = 132;  // floats; rows of 128 start in different banks
 
 template <int HD, int NC>
 struct FewLayout {
-  static constexpr int NH = HD / 64, NS = HD == 128 ? (NC == 16 ? 6 : 5) : 10;
+  static constexpr int NH = HD / 64, NS = HD == 128 ? (NC == 16 ? 6 : 5) : (NC == 16 ? 10 : 9);
   static constexpr uint32_t TILE = NH * kHalf;
   static constexpr uint32_t QB = NH * NC * 128;  // one Q buffer
-  static constexpr uint32_t PB = 2 * NC * 128;   // one P^T buffer
+  static constexpr uint32_t PB = 2 * NC * 128;   // one P^T buffer's high or low parts
   static constexpr uint32_t Q = NS * TILE;       // two buffers: the next piece's Q comes early
   static constexpr uint32_t P = Q + 2 * QB;
-  static constexpr uint32_t RED = P + 2 * PB;    // float [4][NC]
+  static constexpr uint32_t RED = P + 4 * PB;    // float [4][NC]
   static constexpr uint32_t SUMS = RED + 4 * NC * 4;  // float [NC][kSumStride]
   static constexpr uint32_t BARS = SUMS + NC * kSumStride * 4;
   // (at HD = 64 an MMA's second 64-wide block lies one half tile further on, past the last stage's end)
@@ -208,15 +215,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         if (!(ok = wait_warp(&bars->full[st], (item / NS) & 1, abort_flag))) break;
         if (!(ok = wait_warp(&bars->p_full[pb], (it >> 1) & 1, abort_flag))) break;
         tc_fence_after();
-        const uint64_t v_desc = sw128_desc(base + st * L::TILE, kHalf, 1024), p_desc = sw128_desc(base + L::P + pb * L::PB, 16, 1024);
+        const uint64_t v_desc = sw128_desc(base + st * L::TILE, kHalf, 1024), p_desc = sw128_desc(base + L::P + pb * 2 * L::PB, 16, 1024);
         if (elect_one()) {
           // A = V^T: rows of the tile are keys (the K axis), head dims contiguous;
           // at HD = 64 rows 64 .. 127 of the product come from the bytes after
           // the tile and are not read
 #pragma unroll
-          for (int kk = 0; kk < kTileKeys / 16; ++kk)
-            mma_f16_ss(tmem + 2 * NC, desc_at(v_desc, kk * 16 * 128), desc_at(p_desc, (kk >> 2) * NC * 128 + (kk & 3) * 32),
-                       IDESC_PV, t > 0 || kk > 0);
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int kk = 0; kk < kTileKeys / 16; ++kk)
+              mma_f16_ss(tmem + 2 * NC, desc_at(v_desc, kk * 16 * 128),
+                         desc_at(p_desc, part * L::PB + (kk >> 2) * NC * 128 + (kk & 3) * 32), IDESC_PV,
+                         t > 0 || part > 0 || kk > 0);
           mma_commit(&bars->empty[st]);
           mma_commit(&bars->p_empty[pb]);
           if (t + 1 == nt) mma_commit(&bars->o_full);
@@ -328,13 +338,15 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           }
         }
         if (ok) ok = wait_warp(&bars->p_empty[sb], ((it >> 1) & 1) ^ 1, abort_flag);
-        const uint32_t dst = p_base + sb * L::PB + p_half + p_in;
+        const uint32_t dst = p_base + sb * 2 * L::PB + p_half + p_in;
 #pragma unroll
         for (int e = 0; e < NC; ++e) {
           const float v = ex2_ftz(x[e] - m[e]);
           l[e] += v;
-          const T y = from_f32<T>(v);
-          sts_u16(dst + e * 128 + ((p_chunk ^ (e & 7)) << 4), *reinterpret_cast<const uint16_t*>(&y));
+          const T hi = from_f32<T>(v), lo = from_f32<T>(v - to_f32<T>(hi));
+          const uint32_t at = dst + e * 128 + ((p_chunk ^ (e & 7)) << 4);
+          sts_u16(at, *reinterpret_cast<const uint16_t*>(&hi));
+          sts_u16(at + L::PB, *reinterpret_cast<const uint16_t*>(&lo));
         }
         if (kb + kTileKeys > u.g.k_len) {
           // V rows past the sequence: zeroed, since 0 x NaN would reach O

@@ -325,6 +325,33 @@ def _stale_results(b):
     del junk
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,new", [(4, [1, 1]), (8, [4, 1])])
+def test_decoding_rounds_the_result_only(group, new, dim, dtype):
+    """Few rows: P goes into P V as two 16-bit parts, whose sum is off by U^2 (and by float16's least step 2^-25 of the largest)."""
+    b = Batch(new, [5000, 700], seed=57, group=group, hkv=2, dim=dim, dtype=dtype)
+    out = b.chunk("softmax1")
+    want, loose, _, _ = b.expected("softmax1")
+    u = UNIT[dtype]
+    q_all, kc, vc = b.query.double().numpy(), b.key_cache.double().numpy(), b.value_cache.double().numpy()
+    tol = np.zeros(want.shape)
+    for s, (n, c) in enumerate(zip(b.new, b.lens)):
+        rows = b.rows[s].numpy()
+        for h in range(want.shape[1]):
+            k, v = kc[rows, h // group], np.abs(vc[rows, h // group])
+            for i in range(n):
+                t, see = int(b.cu[s]) + i, c - n + i + 1
+                x = dim ** -0.5 * (k[:see] @ q_all[t, h])
+                p = np.exp(x) / (1.0 + np.exp(x).sum())
+                ds = 4 * math.sqrt(dim) * 2.0 ** -24 * dim ** -0.5 * (np.abs(k[:see]) @ np.abs(q_all[t, h])).max()
+                step = 2.0 ** -25 * max(p.max(), 0.0) if dtype is torch.float16 else 0.0
+                # (the float32 sums of see products: 1e-6 of the largest value, as in expected())
+                tol[t, h] = 1.01 * u * np.abs(want[t, h]) + (u * u + 2 * ds) * (p @ v[:see]) + step * v[:see].sum(0) \
+                    + 1e-6 * v[:see].max()
+    _check(out, want, tol, "out")
+
+
 @pytest.mark.parametrize("hint", [0, 2])
 @pytest.mark.parametrize("norm", NORMS)
 @pytest.mark.parametrize("kw", [dict(), dict(dtype=torch.float32), dict(dim=40), dict(page=5), dict(group=48, hkv=1),
