@@ -101,11 +101,15 @@ __device__ __forceinline__ void load_key_tile_tma(uint8_t* stage, const CUtensor
 
 // ------------------------------------------------------------------ host
 inline int sm_count() {
-  static int n[64] = {0};
-  int dev = 0;
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n[dev];
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // Lets `kernel` use `smem` bytes of dynamic shared memory: once per kernel and
