@@ -233,7 +233,7 @@ class PagedServingCache:
         self.lengths = [0] * num_sequences
         self._pages: list[list[int]] = [[] for _ in range(num_sequences)]
         self._free = list(range(num_blocks - 1, -1, -1))
-        self._device = torch.device(device)
+        self._device = self.layers[0].device if self.layers else torch.device(device)
 
     def step(self, new_tokens: Sequence[int]) -> ServingStep:
         """Allocate pages for ``new_tokens[b]`` more tokens of every sequence (0: the sequence rests)."""

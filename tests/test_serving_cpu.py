@@ -103,3 +103,12 @@ def test_fake_tensors(grad):
         assert out.shape == (3, 4, 64) and out.dtype is torch.bfloat16 and out.device.type == "cuda"
         lens, kept = serving.paged_evict(kc, vc, w, table, lens, 16, 10)
         assert lens.shape == (2,) and kept.shape == (2, 2, 10) and kept.dtype is torch.int32
+
+
+def test_cache_on_the_device_of_its_pages():
+    """A cache made for "cuda" stays with the device that was current then."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        cache = serving.PagedServingCache(1, 2, 4, 16, 1, 64)
+        assert cache._device == cache.layers[0].device and cache._device.index is not None
