@@ -219,8 +219,10 @@ class PagedServingCache:
 
     ``step`` gives every sequence room for its new tokens; ``append`` and
     ``attend`` are called once per layer of that step; ``evict`` cuts every
-    sequence to a budget and returns the freed pages.  Lengths follow from what
-    the host has asked for, so no call waits for the GPU.
+    sequence to a budget and returns the freed pages; ``release`` ends one.
+    Lengths follow from what the host has asked for, so no call waits for the
+    GPU.  ``lengths`` count cached keys: after an eviction a text's positions
+    (of its rotary embedding, say) run ahead of them, and the caller keeps them.
     """
 
     def __init__(self, num_layers: int, num_sequences: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int,
@@ -248,6 +250,14 @@ class PagedServingCache:
             self._pages[b].extend(self._free.pop() for _ in range(n))
             self.lengths[b] += new_tokens[b]
         return self._describe(new_tokens)
+
+    def release(self, sequence: int) -> None:
+        """End a sequence: its pages are free, and its place takes a new text with the next step."""
+        if not 0 <= sequence < len(self.lengths):
+            raise ValueError(f"The cache has no sequence {sequence}.")
+        self._free.extend(reversed(self._pages[sequence]))
+        self._pages[sequence] = []
+        self.lengths[sequence] = 0
 
     def _describe(self, new_tokens: Sequence[int]) -> ServingStep:
         width = max(1, max(len(p) for p in self._pages))

@@ -112,3 +112,23 @@ def test_cache_on_the_device_of_its_pages():
     with FakeTensorMode():
         cache = serving.PagedServingCache(1, 2, 4, 16, 1, 64)
         assert cache._device == cache.layers[0].device and cache._device.index is not None
+
+
+def test_release_ends_one_sequence():
+    """Its pages go to others, and its place takes a new text."""
+    cache = serving.PagedServingCache(1, 3, 6, 16, 1, 64, device="cpu")
+    cache.step([40, 16, 20])
+    with pytest.raises(ValueError, match="no room"):
+        cache.step([0, 16, 0])
+    cache.release(0)
+    assert cache.lengths == [0, 16, 20]
+    step = cache.step([5, 16, 13])
+    assert cache.lengths == [5, 32, 33] and step.lengths.tolist() == [5, 32, 33]
+    used = [p for b, n in enumerate((1, 2, 3)) for p in step.block_table[b, :n].tolist()]
+    assert sorted(used) == list(range(6))
+    cache.release(1)
+    cache.release(1)  # nothing left to free
+    assert cache.step([0, 0, 31]).max_seqlen_k == 64
+    for b in (3, -1):
+        with pytest.raises(ValueError, match="no sequence"):
+            cache.release(b)
