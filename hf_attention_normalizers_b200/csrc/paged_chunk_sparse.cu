@@ -13,7 +13,11 @@
 //
 // Rows with more live candidates than the buffer holds are solved by bracket
 // sweeps over all keys; a CTA with such a row leaves its P V to the dense
-// kernel (its flag tells it to), which has tau from the statistics.
+// kernel (its flag tells it to), which has tau from the statistics.  That is a
+// matter of the scores: entmax15, 4 x 256 tokens on 8k keys, takes 223 us with
+// queries of twice unit deviation (supports of 8-10 keys), 260 at 1.5 and 862 at
+// unit deviation (about 25 keys, and nearly every unit has a row over the
+// buffer); sparsemax 139, 146 and 158.
 //
 // Measured: sparsemax, 4 x up to 256 tokens on up to 8k keys: 85 us, of a CTA's
 // 118k cycles 73k in the scan, 9k in the threshold, 29k in the gather.  The scan
@@ -626,7 +630,12 @@ cudaError_t run_norm(const AttnParams& p, const ChunkPlan& c, int ranks, int* fl
 
 cudaError_t chunk_sparse_scan(int dtype, const AttnParams& p, const ChunkPlan& c, int* flags, cudaStream_t s) {
   // CTAs of a cluster: up to two waves over the SMs (the bound counts pairs
-  // that ragged sequences do not fill), each CTA with four key tiles or more
+  // that ragged sequences do not fill), each CTA with four key tiles or more.
+  // Measured with 1 / 2 / 4 / 8 ranks (sparsemax, 8 KV heads, us; entmax15 alike):
+  // 1 token on 32k keys 266 / 153 / 96 / 69 (the rule: 8), 4 x 1 on 2k 42 / 37 /
+  // 34 / 72 (4), 8 x 1 on 8k 92 / 67 / 92 / 170 (2), 4 x 256 on 8k 140 / 179 /
+  // 240 / 419 (1).  A bound that is not reached costs: 2 x 130 tokens on 3k take
+  // 83 / 63 / 87 / 129, and the rule says 4.
   const int64_t units = (int64_t)c.pairs * p.hkv, ktiles = (p.len_k + kTileKeys - 1) / kTileKeys;
   int ranks = 1;
   while (ranks < kMaxCluster && units * ranks <= sm_count() && ktiles >= ranks * 8) ranks *= 2;

@@ -58,6 +58,9 @@ using namespace tc;
 
 constexpr int kChunkThreads = 352;
 constexpr int kMaxRing = 8;
+// (bfloat16, a mixed batch of 452 tokens / 4 x 256 on 8k keys, us: 2^4 100 / 183,
+// 2^8 90 / 162, 2^12 91 / 161, 2^20 91 / 161; scores of four times unit
+// deviation: 106 / 200, 100 / 187, 95 / 170, 99 / 194)
 template <bool BF16>
 constexpr float kHighSum = BF16 ? 4096.f : 32768.f;  // (also keeps P below float16's 65504)
 // Factor of s - tau: float16 takes the sparse normalizers' P (at most 1) times

@@ -501,12 +501,21 @@ int few_columns(const AttnParams& p) {
 
 }  // namespace
 
-constexpr int64_t kFewScoreBytes = 1ll << 30;  // scores kept at most; beyond, the weights read K again
+// Scores kept at most; beyond, the weights read K again.  A bound on memory, not
+// on time: kept scores stay ahead (0.25 GiB, 64 x 1 token on 32k keys: 1504
+// against 3278 us; 0.5 GiB, 64 x 8 tokens on 8k: 726 against 818).
+constexpr int64_t kFewScoreBytes = 1ll << 30;
 
 static int64_t score_bytes(const AttnParams& p, const ChunkPlan& c) {
   return (int64_t)p.rows_total * p.hkv * p.len_k * score_floats(c.group) * 4;
 }
 
+// Against the dense kernel, both measured (8 KV heads, us, few / dense): up to 16
+// packed rows ahead everywhere (1 token on 32k keys 49 / 51, 32 x 1 on 8k 194 /
+// 213, 16 x 4 tokens of 4 heads on 8k 115 / 121; with weights 54 / 82, 220 / 442,
+// 148 / 238).  17 to 32 rows: behind without weights (16 x 4 tokens of 8 heads on
+// 8k 125 / 117, 1 x 4 on 32k 70 / 59), mostly ahead with them (217 / 235, 104 /
+// 89); they run here for P in two parts.
 bool chunk_few_applies(const AttnParams& p, const ChunkPlan& c, bool weights) {
   if (p.norm != HFAN_SOFTMAX1 || few_columns(p) == 0) return false;
   return !weights || score_bytes(p, c) <= kFewScoreBytes;

@@ -145,10 +145,12 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
 
     The causal mask is aligned to each sequence's end (its new tokens are its
     last keys); rows that see no key give zeros, and so do the packed rows that
-    no sequence owns (padding before the first offset or past the last).  Cache slots past a sequence's
-    length are never used, whatever they hold.  With ``key_weights`` the
-    probabilities of every key, summed over the new tokens and the query heads
-    of its KV head, are added to its accumulator.
+    no sequence owns (padding before the first offset or past the last).  Cache
+    slots past a sequence's length are never used, whatever they hold; a value
+    row inside it that is not finite may reach rows of the call that the mask
+    hides it from (0 x inf).  With ``key_weights`` the probabilities of every
+    key, summed over the new tokens and the query heads of its KV head, are
+    added to its accumulator.
     """
     _check_cache(key_cache, value_cache, block_table, sequence_lengths, block_size, key_weights,
                  "paged_chunk_attention")

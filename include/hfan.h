@@ -280,7 +280,8 @@ int hfan_paged_chunk_fwd(const hfan_chunk_desc* desc, hfan_tensor q, hfan_tensor
                          int64_t workspace_bytes, void* stream);
 
 /* Writes the new tokens' K/V rows to their slots and zeroes the slots' key
- * weights (key_weights may be NULL).  normalizer, heads_q and scale are ignored. */
+ * weights (key_weights may be NULL).  normalizer and heads_q have to be valid
+ * (0 and heads_kv will do) but say nothing here; scale is ignored. */
 int hfan_paged_append(const hfan_chunk_desc* desc, hfan_tensor k, hfan_tensor v, hfan_tensor key_cache,
                       hfan_tensor value_cache, float* key_weights, int64_t ld_weights, void* stream);
 
@@ -291,7 +292,8 @@ int hfan_paged_append(const hfan_chunk_desc* desc, hfan_tensor k, hfan_tensor v,
  * positions 0 .. budget - 1; later positions keep what they held.  kept: int32
  * [batch, heads_kv, budget] former positions (-1 past a shorter sequence);
  * new_lens: int32 [batch].  Pages must belong to one sequence only.
- * cu_seqlens_q, total_q, normalizer, heads_q and scale are ignored. */
+ * normalizer, heads_q and total_q have to be valid (0, heads_kv and 0 will do)
+ * but say nothing here; cu_seqlens_q and scale are ignored. */
 int hfan_paged_evict(const hfan_chunk_desc* desc, hfan_tensor key_cache, hfan_tensor value_cache, float* key_weights,
                      int64_t ld_weights, int32_t budget, int32_t recent, int32_t* kept, int32_t* new_lens, void* stream);
 
