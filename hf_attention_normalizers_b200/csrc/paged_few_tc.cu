@@ -83,6 +83,10 @@ static_assert(sizeof(FewBars) <= 512, "FewBars outgrew its place");
 static_assert(FewLayout<128, 16>::TOTAL <= 232448 && FewLayout<128, 32>::TOTAL <= 232448 &&
                   FewLayout<64, 16>::TOTAL <= 232448 && FewLayout<64, 32>::TOTAL <= 232448,
               "more shared memory than a block can have");
+// The library's kernels with TMEM take 48 KB of shared memory or more, an SM has 228 KB.
+static_assert(FewLayout<128, 16>::TOTAL > 180 * 1024 && FewLayout<128, 32>::TOTAL > 180 * 1024 &&
+                  FewLayout<64, 16>::TOTAL > 180 * 1024 && FewLayout<64, 32>::TOTAL > 180 * 1024,
+              "a kernel that waits for TMEM could share an SM with blocks that hold some and wait for it");
 
 // Kept scores: [KV head][key][score_floats(rows of the group)] for every group of
 // tokens, rows rounded up to whole vectors.  A token has room for the rounded
@@ -138,6 +142,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     bars->abort = bars->never = 0;
     fence_barrier_init();
   }
+  // (TMEM held while waiting for the predecessor: one that still has to allocate
+  // its own cannot be on this SM, see the assertion on FewLayout)
   if (warp == 5) tmem_alloc(&bars->tmem, 128);
   wait_for_predecessor();
   Walk walk(p, c.tpb);
