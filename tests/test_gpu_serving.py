@@ -417,6 +417,14 @@ def test_rows_that_attend_to_almost_nothing(dtype, new, dim, profile):
 
 
 @pytest.mark.parametrize("norm", ["sparsemax", "entmax15"])
+@pytest.mark.parametrize("kw", [dict(dtype=torch.float32), dict(dim=40), dict(dim=64), dict(dtype=torch.float16, page=5)])
+@pytest.mark.parametrize("gain", [0.1, 1.0])
+def test_nearly_even_rows(gain, kw, norm):
+    """Scores so close that every key is in the support, on every route."""
+    _chunk_case(Batch([7, 1, 30], [2471, 720, 735], seed=65, hkv=1, gain=gain, **kw), norm, scale=1e-3)
+
+
+@pytest.mark.parametrize("norm", ["sparsemax", "entmax15"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_supports_of_very_many_keys(norm, dtype):
     """Even rows over a long context: every probability lies among float16's subnormal numbers."""
