@@ -86,22 +86,28 @@ def _check_rows(rows, key_cache, cu_seqlens, block_table, name) -> None:
         raise ValueError("New tokens and cache head dimensions must match.")
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_compiling, _grad_enabled = torch.compiler.is_compiling, torch.is_grad_enabled
+_modes, _functorch = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
+_profiling = torch._C._autograd._profiler_enabled
+_Tensor, _Parameter = torch.Tensor, torch.nn.Parameter
 
 
 def _check_placement(*tensors) -> bool:
     """Returns whether somebody listens for the call: it is then dispatched as a custom op, else launched directly
     (the dispatch costs as much host time as the launch)."""
     where = tensors[0].get_device()
-    observed = (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-                or torch._C._functorch.peek_interpreter_stack() is not None or torch._C._autograd._profiler_enabled())
+    observed = _compiling() or _modes() > 0 or _functorch() is not None or _profiling()
+    grad = _grad_enabled()
     for t in tensors:
-        if t is not None:
-            if t.get_device() != where:
-                raise ValueError("All tensors must be on one device.")
-            observed = observed or type(t) not in _PLAIN
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("Paged serving is inference only: call it under torch.no_grad() or detach its inputs.")
+        if t is None:
+            continue
+        if t.get_device() != where:
+            raise ValueError("All tensors must be on one device.")
+        if grad and t.requires_grad:
+            raise ValueError("Paged serving is inference only: call it under torch.no_grad() or detach its inputs.")
+        kind = type(t)
+        if kind is not _Tensor and kind is not _Parameter:
+            observed = True
     return observed
 
 
